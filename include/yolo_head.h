@@ -60,6 +60,16 @@ extern "C" {
 #define YH_OP_MAP 4 /* batch = number of predictions */
 #define YH_OP_LOSS_PIPELINED 5
 
+/* number types of the entry points that take more than fp32 */
+#define YH_F32 0
+#define YH_F16 1
+#define YH_BF16 2
+#define YH_I8 3
+
+#define YH_MAX_I8_K 131071   /* yh_linear_i8: 128 * 128 * K stays below 2^31 */
+#define YH_MAX_NS_STEPS 64   /* yh_orthogonalize, yh_muon_step */
+#define YH_MUON_MAX_COUNT 32 /* matrices of one yh_muon_step call */
+
 /* candidate modes of the NMS entry points */
 #define YH_MODE_REFERENCE 0 /* per cell the higher-confidence predictor (model.py:384-390) */
 #define YH_MODE_DENSE 1     /* every predictor of every cell */
@@ -455,6 +465,70 @@ int yh_nms_ws(const float* cand_ltrb, const float* cand_score, const int32_t* ca
               const uint8_t* cand_present, float* dets, int32_t* keep_count, int32_t* keep_idx,
               float conf_thresh, float iou_thresh, int64_t batch, int N, void* workspace,
               size_t workspace_bytes, void* stream);
+
+/*
+ * The product of a linear layer in 8-bit integers, for serving the layers in front of the
+ * head (model.py:133-135): y = s_m * t_n * sum_k q_mk * w_nk + bias_n.  The reference has no
+ * quantised path; its nn.Linear in fp32 is what y approximates.
+ *
+ * yh_quantize_rows: s_m = max_k |x_mk| / 127 and q_mk = 127 * x_mk / max_k |x_mk| rounded to the
+ * nearest whole number, ties to even (the exact quotient decides).  A row of zeros gets the
+ * scale 0; a row that holds a NaN or an infinity gets the scale NaN and zeros.  x (rows, K) of
+ * x_dtype (YH_F32, YH_F16, YH_BF16), ldx numbers from row to row; q (rows, K) int8, ldq bytes from
+ * row to row, q 16-byte aligned, ldq a multiple of 16; the bytes from K to the next multiple of 128
+ * (at most ldq) are written as zeros.  scale (rows) fp32.
+ *
+ * yh_linear_i8: x (M, K), ldx numbers from row to row: YH_F32, YH_F16 or YH_BF16 with x_scale NULL
+ * (quantised as yh_quantize_rows does, in the workspace), or YH_I8 with x_scale (M).  w (N, K) int8,
+ * 16-byte aligned, ldw a multiple of 16, every row readable up to the next multiple of 16 bytes
+ * (what lies there does not matter); w_scale (N) fp32; bias (N) fp32 or NULL.  y (M, N) of y_dtype
+ * (YH_F32, YH_F16, YH_BF16), ldy numbers from row to row.  The sum is exact in int32 (K <=
+ * YH_MAX_I8_K), scales and bias are applied in fp32, the result is rounded once; bitwise
+ * reproducible.  No gradient.
+ * With YH_F32 and no bias y is the z of yh_decode_nms_linear.
+ * workspace: yh_linear_i8_workspace_bytes bytes, 256-byte aligned, contents never matter.
+ */
+int yh_quantize_rows(const void* x, int x_dtype, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
+                     int64_t rows, int64_t K, void* stream);
+size_t yh_linear_i8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int yh_linear_i8(const void* x, int x_dtype, int64_t ldx, const float* x_scale, const int8_t* w,
+                 int64_t ldw, const float* w_scale, const float* bias, void* y, int y_dtype,
+                 int64_t ldy, int64_t M, int64_t N, int64_t K, void* workspace,
+                 size_t workspace_bytes, void* stream);
+
+/*
+ * Orthogonalised updates for the weights of the layers in front of the head (the reference
+ * trains them with AdamW, train.py:84-94).
+ *
+ * yh_orthogonalize: `steps` Newton-Schulz steps X <- (a + b XX' + c (XX')^2) X from
+ * X = G / (|G| + eps), |G| the Frobenius norm, for each of `count` matrices (rows, cols) of g;
+ * a matrix taller than wide is worked on transposed, which changes nothing in exact arithmetic.
+ * g and out of YH_F32, YH_F16 or YH_BF16; g_stride / out_stride numbers from matrix to matrix, ldg /
+ * ldo from row to row, columns next to each other; out must not overlap g or itself.  The matrices are held in
+ * 22 bits and summed in fp32: the result is within about 1e-4 of the exact one (relative, whole
+ * matrix; YH_F32 results 3e-5) before it is rounded to out_dtype, for coefficients that keep the
+ * singular values below 2 (a = 3.4445, b = -4.7750, c = 2.0315 do).  Two calls give the same bits.  A NaN or an
+ * infinity in a matrix makes all of its result NaN; zeros give zeros.
+ *
+ * yh_muon_step: for each of count <= YH_MUON_MAX_COUNT weight matrices (rows, cols) of one shape,
+ * contiguous, in place: m <- momentum * m + g;  u = g + momentum * m (nesterov) or m;
+ * p <- (1 - lr * weight_decay) * p - lr * scale * orthogonalised(u).  params of p_dtype, grads of
+ * g_dtype, momenta fp32.  The three arrays of pointers are read on the host during the call; the pointers
+ * and numbers are what a captured graph replays.  No two params or momenta may overlap.
+ *
+ * workspace (both): yh_orthogonalize_workspace_bytes bytes, 256-byte aligned, contents never
+ * matter.  Limits: the shorter side <= 32,768, the longer <= 2^24, steps <= YH_MAX_NS_STEPS.
+ */
+size_t yh_orthogonalize_workspace_bytes(int64_t count, int64_t rows, int64_t cols);
+int yh_orthogonalize(const void* g, int g_dtype, int64_t g_stride, int64_t ldg, void* out,
+                     int out_dtype, int64_t out_stride, int64_t ldo, int64_t count, int64_t rows,
+                     int64_t cols, float a, float b, float c, int steps, float eps, void* workspace,
+                     size_t workspace_bytes, void* stream);
+int yh_muon_step(void* const* params, int p_dtype, const void* const* grads, int g_dtype,
+                 float* const* momenta, int count, int64_t rows, int64_t cols, float lr,
+                 float momentum, int nesterov, float weight_decay, float scale, float a, float b,
+                 float c, int steps, float eps, void* workspace, size_t workspace_bytes,
+                 void* stream);
 
 #ifdef __cplusplus
 }

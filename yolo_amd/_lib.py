@@ -36,6 +36,16 @@ YH_OP_LOSS_PIPELINED = 5
 YH_MODE_REFERENCE = 0
 YH_MODE_DENSE = 1
 
+YH_F32 = 0
+YH_F16 = 1
+YH_BF16 = 2
+YH_I8 = 3
+DTYPE_CODES = {torch.float32: YH_F32, torch.float16: YH_F16, torch.bfloat16: YH_BF16, torch.int8: YH_I8}
+
+YH_MAX_I8_K = 131071
+YH_MAX_NS_STEPS = 64
+YH_MUON_MAX_COUNT = 32
+
 YH_MAX_CANDIDATES = 2048
 YH_MAX_CANDIDATES_WS = 65536
 YH_STATIC_SCRATCH_BYTES = 262144
@@ -118,6 +128,19 @@ SIGNATURES = {
                                  c_void_p]),
     "yh_nms_ws": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                           c_float, c_float, c_int64, c_int, c_void_p, c_size_t, c_void_p]),
+    "yh_quantize_rows": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64,
+                                 c_void_p]),
+    "yh_linear_i8_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "yh_linear_i8": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
+                             c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_size_t,
+                             c_void_p]),
+    "yh_orthogonalize_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "yh_orthogonalize": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_int, c_int64, c_int64,
+                                 c_int64, c_int64, c_int64, c_float, c_float, c_float, c_int, c_float,
+                                 c_void_p, c_size_t, c_void_p]),
+    "yh_muon_step": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int64, c_int64, c_float,
+                             c_float, c_int, c_float, c_float, c_float, c_float, c_float, c_int, c_float,
+                             c_void_p, c_size_t, c_void_p]),
     "yh_nms": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                        c_float, c_float, c_int64, c_int, c_void_p]),
 }

@@ -1,0 +1,165 @@
+// yh_quantize_rows and yh_linear_i8: the 8-bit product entry points of include/yolo_head.h.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/yolo_head.h"
+#include "linear_i8_kernels.hpp"
+
+namespace {
+
+using namespace yh;
+
+inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+inline size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+inline int launch_status() {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? YH_OK : (int)e;
+}
+inline size_t dtype_bytes(int dt) { return dt == YH_F32 ? 4 : dt == YH_I8 ? 1 : 2; }
+
+constexpr int64_t kMaxRows = ((int64_t)1 << 22) - 1;      // a grid holds fewer than 2^32 threads, a row takes up to 1,024
+
+template <int DT>
+void quantize_launch(const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int K, int Kz,
+                     hipStream_t st) {
+    typedef typename Elem<DT>::T T;
+    const int vec = aligned(x, 16) && (ldx * sizeof(T)) % 16 == 0;
+    if (K > 8192)
+        hipLaunchKernelGGL((quantize_rows_kernel<DT, 1024>), dim3((unsigned)rows), dim3(1024), 0, st, (const T*)x, ldx, q,
+                           ldq, scale, K, Kz, vec);
+    else
+        hipLaunchKernelGGL((quantize_rows_kernel<DT, 256>), dim3((unsigned)rows), dim3(256), 0, st, (const T*)x, ldx, q,
+                           ldq, scale, K, Kz, vec);
+}
+
+int quantize(const void* x, int dt, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int K, int Kz,
+             hipStream_t st) {
+    if (dt == YH_F32) quantize_launch<DT_F32>(x, ldx, q, ldq, scale, rows, K, Kz, st);
+    else if (dt == YH_F16) quantize_launch<DT_F16>(x, ldx, q, ldq, scale, rows, K, Kz, st);
+    else quantize_launch<DT_BF16>(x, ldx, q, ldq, scale, rows, K, Kz, st);
+    return launch_status();
+}
+
+// How the product is cut: tiles of BM x BN and slices of the contraction
+struct Plan {
+    int tiles_m, tiles_n, slices, per_slice, blocks;
+    size_t q_off, s_off, p_off, total;
+};
+
+Plan plan_for(int64_t M, int64_t N, int64_t K) {
+    Plan p = {};
+    p.blocks = (int)((K + 127) / 128);
+    p.tiles_m = (int)((M + 127) / 128);
+    p.tiles_n = (int)((N + 127) / 128);
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+    int64_t s = tiles >= 256 ? 1 : (512 + tiles - 1) / tiles;
+    if (s > (p.blocks + 3) / 4) s = (p.blocks + 3) / 4;
+    if (s < 1) s = 1;
+    p.per_slice = (int)((p.blocks + s - 1) / s);
+    p.slices = (p.blocks + p.per_slice - 1) / p.per_slice;
+    p.q_off = 0;
+    p.s_off = up256((size_t)M * p.blocks * 128);
+    p.p_off = p.s_off + up256((size_t)M * 4);
+    p.total = p.p_off + (p.slices > 1 ? up256((size_t)p.slices * M * N * 4) : 0);
+    return p;
+}
+
+template <int DT>
+int product(const LinearI8Args& a, hipStream_t st) {
+    typedef TileProduct<MathI8, 128, 128, 2, 2, true> P;
+    const unsigned grid = (unsigned)((int64_t)a.tiles_m * a.tiles_n * a.slices);
+    hipLaunchKernelGGL((linear_i8_tile_kernel<DT, 128, 128, 2, 2>), dim3(grid), dim3(P::THREADS), P::LDS_BYTES, st, a);
+    if (const int rc = launch_status()) return rc;
+    if (a.slices > 1) {
+        int64_t b = (a.M * ((a.N + 3) / 4) + 255) / 256;
+        if (b > 4096) b = 4096;
+        hipLaunchKernelGGL((linear_i8_join_kernel<DT>), dim3((unsigned)b), dim3(256), 0, st, a);
+    }
+    return launch_status();
+}
+
+int check_sizes(int64_t M, int64_t N, int64_t K) {
+    if (M < 0 || N < 0 || K < 1 || K > YH_MAX_I8_K || M > kMaxRows || N > kMaxRows) return YH_ERR_SHAPE;
+    if (((M + 127) / 128) * ((N + 127) / 128) >= ((int64_t)1 << 24)) return YH_ERR_SHAPE;
+    return YH_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int yh_quantize_rows(const void* x, int x_dtype, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows,
+                     int64_t K, void* stream) {
+    if (rows < 0 || rows > kMaxRows || K < 1 || K > YH_MAX_I8_K || ldx < K || ldq < K) return YH_ERR_SHAPE;
+    if (x_dtype != YH_F32 && x_dtype != YH_F16 && x_dtype != YH_BF16) return YH_ERR_ARG;
+    if (rows == 0) return YH_OK;
+    if (!x || !q || !scale) return YH_ERR_NULL;
+    if (!aligned(x, dtype_bytes(x_dtype)) || !aligned(scale, 4) || !aligned(q, 16) || ldq % 16 != 0) return YH_ERR_ALIGN;
+    int64_t Kz = (K + 127) / 128 * 128;
+    if (Kz > ldq) Kz = ldq;
+    return quantize(x, x_dtype, ldx, q, ldq, scale, rows, (int)K, (int)Kz, (hipStream_t)stream);
+}
+
+size_t yh_linear_i8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    if (check_sizes(M, N, K) != YH_OK || M == 0 || N == 0) return 0;
+    return plan_for(M, N, K).total;
+}
+
+int yh_linear_i8(const void* x, int x_dtype, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw,
+                 const float* w_scale, const float* bias, void* y, int y_dtype, int64_t ldy, int64_t M, int64_t N,
+                 int64_t K, void* workspace, size_t workspace_bytes, void* stream) {
+    if (const int rc = check_sizes(M, N, K)) return rc;
+    if (ldx < K || ldw < K || ldy < N) return YH_ERR_SHAPE;
+    if (x_dtype < YH_F32 || x_dtype > YH_I8 || y_dtype < YH_F32 || y_dtype > YH_BF16) return YH_ERR_ARG;
+    if ((x_dtype == YH_I8) != (x_scale != nullptr)) return YH_ERR_ARG;
+    if (M == 0 || N == 0) return YH_OK;
+    if (!x || !w || !w_scale || !y) return YH_ERR_NULL;
+    const Plan p = plan_for(M, N, K);
+    if (!workspace || workspace_bytes < p.total) return YH_ERR_WORKSPACE;
+    if (!aligned(x, dtype_bytes(x_dtype)) || !aligned(x_scale, 4) || !aligned(w, 16) || ldw % 16 != 0 ||
+        !aligned(w_scale, 4) || !aligned(bias, 4) || !aligned(y, dtype_bytes(y_dtype)) || !aligned(workspace, 256))
+        return YH_ERR_ALIGN;
+    hipStream_t st = (hipStream_t)stream;
+    char* ws = (char*)workspace;
+    LinearI8Args a = {};
+    a.q = (const int8_t*)(ws + p.q_off);
+    a.ldq = (long long)p.blocks * 128;
+    a.sx = (const float*)(ws + p.s_off);
+    if (x_dtype != YH_I8) {
+        const int rc = quantize(x, x_dtype, ldx, (int8_t*)(ws + p.q_off), a.ldq, (float*)(ws + p.s_off), M, (int)K,
+                                (int)a.ldq, st);
+        if (rc) return rc;
+    } else {
+        a.sx = x_scale;
+        if (K % 128 == 0 && ldx % 16 == 0 && aligned(x, 16)) {
+            a.q = (const int8_t*)x;
+            a.ldq = ldx;
+        } else {
+            hipLaunchKernelGGL(repack_rows_kernel, dim3((unsigned)M), dim3(256), 0, st, (const int8_t*)x, ldx,
+                               (int8_t*)(ws + p.q_off), a.ldq, (int)K, (int)a.ldq);
+            if (const int rc = launch_status()) return rc;
+        }
+    }
+    a.w = w;
+    a.ldw = ldw;
+    a.sw = w_scale;
+    a.bias = bias;
+    a.y = y;
+    a.ldy = ldy;
+    a.partial = (int*)(ws + p.p_off);
+    a.M = M;
+    a.N = N;
+    a.last_w = (int)((K + 15) / 16 * 16 - 16);
+    a.blocks = p.blocks;
+    a.slices = p.slices;
+    a.per_slice = p.per_slice;
+    a.tiles_m = p.tiles_m;
+    a.tiles_n = p.tiles_n;
+    a.whole = (ldy * dtype_bytes(y_dtype)) % (4 * dtype_bytes(y_dtype)) == 0 && aligned(y, 4 * dtype_bytes(y_dtype));
+    if (y_dtype == YH_F32) return product<DT_F32>(a, st);
+    if (y_dtype == YH_F16) return product<DT_F16>(a, st);
+    return product<DT_BF16>(a, st);
+}
+
+}  // extern "C"

@@ -1,0 +1,337 @@
+// yh_orthogonalize and yh_muon_step: the entry points of the orthogonalised update (include/yolo_head.h).
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/yolo_head.h"
+#include "orthogonalize_kernels.hpp"
+
+namespace {
+
+using namespace yh;
+
+inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+inline size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+inline int launch_status() {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? YH_OK : (int)e;
+}
+inline size_t dtype_bytes(int dt) { return dt == YH_F32 ? 4 : 2; }
+
+constexpr int64_t kMaxShort = 32768, kMaxLong = (int64_t)1 << 24, kMaxNumbers = (int64_t)1 << 38;
+constexpr int TB = 128;                       // tile of the products
+typedef TileProduct<MathSplit, TB, TB, 2, 2, true> Tile;
+
+// powers of two the split matrices are held at: A and T up to about 1.5, R up to 127, S up to 1023
+constexpr float kScaleA = 512.0f, kScaleR = 512.0f, kScaleS = 64.0f, kScaleX = 4096.0f;
+
+NsShape shape_of(int64_t rows, int64_t cols, int count) {
+    NsShape s = {};
+    s.rows = rows;
+    s.cols = cols;
+    s.tall = rows > cols;
+    s.l = s.tall ? cols : rows;
+    s.n = s.tall ? rows : cols;
+    s.lk = (s.l + 31) & ~31ll;
+    s.nk = (s.n + 31) & ~31ll;
+    s.count = count;
+    return s;
+}
+
+int check_sizes(int64_t count, int64_t rows, int64_t cols) {
+    if (count < 0 || count > 65535 || rows < 1 || cols < 1) return YH_ERR_SHAPE;
+    const int64_t l = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
+    if (l > kMaxShort || n > kMaxLong || l * n > kMaxNumbers) return YH_ERR_SHAPE;
+    // workgroups of a launch (256 threads each; a grid holds fewer than 2^32 threads)
+    if (count > kMaxNumbers / (l * n) || (count < 1 ? 1 : count) * ((l + 63) / 64) * ((n + 63) / 64) >= ((int64_t)1 << 24))
+        return YH_ERR_SHAPE;
+    return YH_OK;
+}
+
+struct Layout {
+    size_t parts, x, xt, xt2, a, r0, r1, t, s0, s1, partial, total;
+    long long x_mat, xt_mat, sq_mat;
+    int norm_blocks, tiles, slices, per_slice;
+};
+
+Layout layout_for(const NsShape& s) {
+    Layout w = {};
+    int64_t nb = (s.rows * s.cols + 4095) / 4096;
+    w.norm_blocks = (int)(nb < 1 ? 1 : nb > NS_NORM_BLOCKS ? NS_NORM_BLOCKS : nb);
+    w.x_mat = s.l * s.nk * 4;
+    w.xt_mat = s.n * s.lk * 4;
+    w.sq_mat = s.l * s.lk * 4;
+    const int64_t side = (s.l + TB - 1) / TB;
+    w.tiles = (int)(side * (side + 1) / 2);
+    // the contraction of X X' is cut when the tiles alone do not fill the card
+    const int64_t blocks = s.nk / 32, wgs = (int64_t)w.tiles * s.count;
+    int64_t cut = wgs >= 256 ? 1 : (512 + wgs - 1) / wgs;
+    if (cut > (blocks + 7) / 8) cut = (blocks + 7) / 8;
+    w.per_slice = (int)((blocks + cut - 1) / cut);
+    w.slices = (int)((blocks + w.per_slice - 1) / w.per_slice);
+    size_t off = 0;
+    auto take = [&](size_t bytes) { const size_t at = off; off += up256(bytes); return at; };
+    w.parts = take((size_t)s.count * w.norm_blocks * 8);
+    w.x = take((size_t)s.count * w.x_mat);
+    w.xt = take((size_t)s.count * w.xt_mat);
+    w.xt2 = take((size_t)s.count * w.xt_mat);
+    w.a = take((size_t)s.count * w.sq_mat);
+    w.r0 = take((size_t)s.count * w.sq_mat);
+    w.r1 = take((size_t)s.count * w.sq_mat);
+    w.t = take((size_t)s.count * w.sq_mat);
+    w.s0 = take((size_t)s.count * w.sq_mat);
+    w.s1 = take((size_t)s.count * w.sq_mat);
+    w.partial = take(w.slices > 1 ? (size_t)w.slices * w.tiles * s.count * TB * TB * 4 : 0);
+    w.total = off;
+    return w;
+}
+
+// where the result goes
+struct Sink {
+    int dtype;
+    void* out;
+    int64_t out_b, out_r;
+    void* const* params;
+    float decay, step;
+};
+
+template <int DT, int OUT, bool TALL>
+int apply(const NsApply& a, hipStream_t st) {
+    const int64_t tiles = ((a.sh.l + TB - 1) / TB) * ((a.sh.n + TB - 1) / TB) * a.sh.count;
+    hipLaunchKernelGGL((ns_apply_kernel<DT, OUT, TALL, TB, TB, 2, 2>), dim3((unsigned)tiles), dim3(Tile::THREADS),
+                       Tile::LDS_BYTES, st, a);
+    return launch_status();
+}
+
+template <int OUT>
+int apply_as(int dt, bool tall, const NsApply& a, hipStream_t st) {
+    if (dt == YH_F32) return tall ? apply<DT_F32, OUT, true>(a, st) : apply<DT_F32, OUT, false>(a, st);
+    if (dt == YH_F16) return tall ? apply<DT_F16, OUT, true>(a, st) : apply<DT_F16, OUT, false>(a, st);
+    return tall ? apply<DT_BF16, OUT, true>(a, st) : apply<DT_BF16, OUT, false>(a, st);
+}
+
+int products(const NsProducts& a, int jobs, hipStream_t st) {
+    const unsigned grid = (unsigned)((int64_t)a.tiles * a.count * a.slices);
+    hipLaunchKernelGGL((ns_product_kernel<TB, 2, 2>), dim3(grid, (unsigned)jobs), dim3(Tile::THREADS), Tile::LDS_BYTES, st, a);
+    if (const int rc = launch_status()) return rc;
+    if (a.slices > 1)
+        hipLaunchKernelGGL((ns_join_kernel<TB, 2, 2>), dim3((unsigned)(a.tiles * a.count)), dim3(Tile::THREADS), 0, st, a);
+    return launch_status();
+}
+
+template <int DT, bool LIST>
+int load(const NsSource& src, const NsShape& s, const Layout& w, char* ws, double eps, double scale, hipStream_t st) {
+    hipLaunchKernelGGL((ns_norm_kernel<DT, LIST>), dim3((unsigned)w.norm_blocks, (unsigned)s.count), dim3(256), 0, st, src, s,
+                       (double*)(ws + w.parts));
+    if (const int rc = launch_status()) return rc;
+    char* x = ws + w.x;
+    char* xt = ws + w.xt;
+    hipLaunchKernelGGL((ns_convert_kernel<DT, LIST>),
+                       dim3((unsigned)(((s.cols + 63) / 64) * ((s.rows + 63) / 64)), (unsigned)s.count), dim3(256), 0, st,
+                       src, s, (const double*)(ws + w.parts), w.norm_blocks, eps, scale, s.tall ? xt : x,
+                       s.tall ? w.xt_mat : w.x_mat, s.tall ? x : xt, s.tall ? w.x_mat : w.xt_mat);
+    return launch_status();
+}
+
+template <bool LIST>
+int load_as(int dt, const NsSource& src, const NsShape& s, const Layout& w, char* ws, double eps, double scale, hipStream_t st) {
+    if (dt == YH_F32) return load<DT_F32, LIST>(src, s, w, ws, eps, scale, st);
+    if (dt == YH_F16) return load<DT_F16, LIST>(src, s, w, ws, eps, scale, st);
+    return load<DT_BF16, LIST>(src, s, w, ws, eps, scale, st);
+}
+
+// G is in the workspace as X and X' (at `scale`); the steps, and the result to `sink`
+int run_steps(const NsShape& s, const Layout& w, char* ws, double scale, float a, float b, float c, int steps, const Sink& sink,
+              hipStream_t st) {
+    char *A = ws + w.a, *T = ws + w.t, *R[2] = {ws + w.r0, ws + w.r1}, *S[2] = {ws + w.s0, ws + w.s1};
+    char *X = ws + w.x, *Xt = ws + w.xt, *Xt_next = ws + w.xt2;
+    const int lb = (int)(s.lk / 32);
+    const double limit = sink.dtype == YH_F32 ? 64.0 : 512.0;
+    NsProducts base = {};
+    base.l = s.l;
+    base.lk = s.lk;
+    base.count = s.count;
+    base.tiles = w.tiles;
+    base.slices = 1;
+    base.per_slice = lb;
+    auto job = [&](const char* P, const char* Q, char* out, float k0, const char* E1, float k1, const char* E2, float k2) {
+        NsProduct p = {};
+        p.P = P;
+        p.Q = Q;
+        p.E1 = E1;
+        p.E2 = E2;
+        p.out = out;
+        p.p_mat = p.out_mat = w.sq_mat;
+        p.ldp = s.lk * 4;
+        p.k0 = k0;
+        p.k1 = k1;
+        p.k2 = k2;
+        p.blocks = lb;
+        return p;
+    };
+    int done = 0;
+    while (done < steps) {
+        int len = 1;
+        for (double grown = fabs((double)a) * fabs((double)a); done + len < steps && grown <= limit; grown *= fabs((double)a)) ++len;
+        // A = X X'
+        NsProducts gram = base;
+        gram.slices = w.slices;
+        gram.per_slice = w.per_slice;
+        gram.partial = (float*)(ws + w.partial);
+        gram.job[0] = job(X, X, A, (float)(kScaleA / (scale * scale)), nullptr, 0.0f, nullptr, 0.0f);
+        gram.job[0].p_mat = w.x_mat;
+        gram.job[0].ldp = s.nk * 4;
+        gram.job[0].blocks = (int)(s.nk / 32);
+        if (const int rc = products(gram, 1, st)) return rc;
+        double q = a;                          // Q = q + S
+        const char* Q = nullptr;
+        float sq = 0.0f;
+        for (int j = 0; j < len; ++j) {
+            char* Rj = R[j & 1];
+            NsProducts one = base;
+            one.job[0] = job(A, A, Rj, c * kScaleR / (kScaleA * kScaleA), A, b * kScaleR / kScaleA, nullptr, 0.0f);
+            if (const int rc = products(one, 1, st)) return rc;
+            int jobs = 0;
+            NsProducts two = base;
+            const bool last = j + 1 == len;
+            if (!last) two.job[jobs++] = job(Rj, A, T, 1.0f / kScaleR, A, a, nullptr, 0.0f);
+            if (j > 0) {
+                two.job[jobs++] = job(Rj, Q, S[j & 1], kScaleS / (kScaleR * sq), Q, a * kScaleS / sq, Rj, (float)(q * kScaleS / kScaleR));
+                q *= a;
+                Q = S[j & 1];
+                sq = kScaleS;
+            } else {
+                Q = Rj;
+                sq = kScaleR;
+            }
+            if (jobs)
+                if (const int rc = products(two, jobs, st)) return rc;
+            if (!last) {
+                NsProducts three = base;
+                three.job[0] = job(T, Rj, A, 1.0f / kScaleR, T, a, nullptr, 0.0f);
+                if (const int rc = products(three, 1, st)) return rc;
+            }
+        }
+        done += len;
+        NsApply ap = {};
+        ap.S = Q;
+        ap.X = X;
+        ap.Xt = Xt;
+        ap.s_mat = w.sq_mat;
+        ap.x_mat = w.x_mat;
+        ap.xt_mat = w.xt_mat;
+        ap.sh = s;
+        ap.k0 = (float)(1.0 / (sq * scale));
+        ap.k1 = (float)(q / scale);
+        if (done < steps) {
+            ap.Yn = X;
+            ap.Yt = Xt_next;
+            ap.again = kScaleX;
+            if (const int rc = apply<DT_F32, NS_OUT_SPLIT, false>(ap, st)) return rc;
+            char* swap = Xt;
+            Xt = Xt_next;
+            Xt_next = swap;
+            scale = kScaleX;
+        } else if (sink.params) {
+            for (int i = 0; i < s.count; ++i) ap.param[i] = sink.params[i];
+            ap.decay = sink.decay;
+            ap.step = sink.step;
+            if (const int rc = apply_as<NS_OUT_WEIGHT>(sink.dtype, s.tall, ap, st)) return rc;
+        } else {
+            ap.out = sink.out;
+            ap.out_b = sink.out_b;
+            ap.out_r = sink.out_r;
+            const size_t e = dtype_bytes(sink.dtype);
+            ap.whole = aligned(sink.out, 4 * e) && sink.out_r % 4 == 0 && sink.out_b % 4 == 0;
+            if (const int rc = apply_as<NS_OUT_RESULT>(sink.dtype, s.tall, ap, st)) return rc;
+        }
+    }
+    return YH_OK;
+}
+
+// X_0 is held at about unit mean square, a spike in it still below fp16's largest number
+double first_scale(const NsShape& s) {
+    int e = (int)floor(0.5 * log2((double)s.rows * (double)s.cols));
+    if (e > 15) e = 15;
+    return ldexp(1.0, e);
+}
+
+bool known(int dt) { return dt == YH_F32 || dt == YH_F16 || dt == YH_BF16; }
+
+}  // namespace
+
+extern "C" {
+
+size_t yh_orthogonalize_workspace_bytes(int64_t count, int64_t rows, int64_t cols) {
+    if (check_sizes(count, rows, cols) != YH_OK || count == 0) return 0;
+    return layout_for(shape_of(rows, cols, (int)count)).total;
+}
+
+int yh_orthogonalize(const void* g, int g_dtype, int64_t g_stride, int64_t ldg, void* out, int out_dtype, int64_t out_stride,
+                     int64_t ldo, int64_t count, int64_t rows, int64_t cols, float a, float b, float c, int steps, float eps,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+    if (const int rc = check_sizes(count, rows, cols)) return rc;
+    if (ldg < cols || ldo < cols || (count > 1 && out_stride < (rows - 1) * ldo + cols)) return YH_ERR_SHAPE;
+    if (!known(g_dtype) || !known(out_dtype)) return YH_ERR_ARG;
+    if (!isfinite(a) || !isfinite(b) || !isfinite(c) || steps < 1 || steps > YH_MAX_NS_STEPS || !(eps >= 0.0f) || isinf(eps))
+        return YH_ERR_ARG;
+    if (count == 0) return YH_OK;
+    if (!g || !out) return YH_ERR_NULL;
+    const NsShape s = shape_of(rows, cols, (int)count);
+    const Layout w = layout_for(s);
+    if (!workspace || workspace_bytes < w.total) return YH_ERR_WORKSPACE;
+    if (!aligned(g, dtype_bytes(g_dtype)) || !aligned(out, dtype_bytes(out_dtype)) || !aligned(workspace, 256)) return YH_ERR_ALIGN;
+    hipStream_t st = (hipStream_t)stream;
+    char* ws = (char*)workspace;
+    NsSource src = {};
+    src.base = g;
+    src.stride_b = g_stride;
+    src.stride_r = ldg;
+    const double scale = first_scale(s);
+    if (const int rc = load_as<false>(g_dtype, src, s, w, ws, eps, scale, st)) return rc;
+    Sink sink = {};
+    sink.dtype = out_dtype;
+    sink.out = out;
+    sink.out_b = out_stride;
+    sink.out_r = ldo;
+    return run_steps(s, w, ws, scale, a, b, c, steps, sink, st);
+}
+
+int yh_muon_step(void* const* params, int p_dtype, const void* const* grads, int g_dtype, float* const* momenta, int count,
+                 int64_t rows, int64_t cols, float lr, float momentum, int nesterov, float weight_decay, float scale, float a,
+                 float b, float c, int steps, float eps, void* workspace, size_t workspace_bytes, void* stream) {
+    if (count < 0 || count > YH_MUON_MAX_COUNT) return YH_ERR_SHAPE;
+    if (const int rc = check_sizes(count, rows, cols)) return rc;
+    if (!known(p_dtype) || !known(g_dtype)) return YH_ERR_ARG;
+    if (!isfinite(lr) || !isfinite(momentum) || !isfinite(weight_decay) || !isfinite(scale) || !isfinite(a) || !isfinite(b) ||
+        !isfinite(c) || steps < 1 || steps > YH_MAX_NS_STEPS || !(eps >= 0.0f) || isinf(eps))
+        return YH_ERR_ARG;
+    if (count == 0) return YH_OK;
+    if (!params || !grads || !momenta) return YH_ERR_NULL;
+    NsSource src = {};
+    for (int i = 0; i < count; ++i) {
+        if (!params[i] || !grads[i] || !momenta[i]) return YH_ERR_NULL;
+        if (!aligned(params[i], dtype_bytes(p_dtype)) || !aligned(grads[i], dtype_bytes(g_dtype)) || !aligned(momenta[i], 4))
+            return YH_ERR_ALIGN;
+        src.g[i] = grads[i];
+        src.buf[i] = momenta[i];
+    }
+    const NsShape s = shape_of(rows, cols, count);
+    const Layout w = layout_for(s);
+    if (!workspace || workspace_bytes < w.total) return YH_ERR_WORKSPACE;
+    if (!aligned(workspace, 256)) return YH_ERR_ALIGN;
+    src.momentum = momentum;
+    src.nesterov = nesterov != 0;
+    hipStream_t st = (hipStream_t)stream;
+    char* ws = (char*)workspace;
+    const double first = first_scale(s);
+    if (const int rc = load_as<true>(g_dtype, src, s, w, ws, eps, first, st)) return rc;
+    Sink sink = {};
+    sink.dtype = p_dtype;
+    sink.params = params;
+    sink.decay = (float)(1.0 - (double)lr * (double)weight_decay);
+    sink.step = (float)((double)lr * (double)scale);
+    return run_steps(s, w, ws, first, a, b, c, steps, sink, st);
+}
+
+}  // extern "C"

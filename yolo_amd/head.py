@@ -22,49 +22,8 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-
-
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
-
-
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-class _on_device:
-    """``torch.cuda.device(dev)`` only when ``dev`` is not already current (the
-    context manager costs several microseconds per call otherwise)."""
-
-    __slots__ = ("ctx",)
-
-    def __init__(self, device):
-        idx = device.index if device.index is not None else torch.cuda.current_device()
-        self.ctx = None if idx == torch.cuda.current_device() else torch.cuda.device(idx)
-
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
-        return False
-
-
-def _need(t: torch.Tensor, name: str, dtype, shape=None) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
-    if not t.is_cuda:
-        raise ValueError(f"{name}: must live on the GPU (got device {t.device}); "
-                         "yolo_amd has no CPU path")
-    if t.dtype != dtype:
-        raise ValueError(f"{name}: expected dtype {dtype}, got {t.dtype}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name}: must be contiguous")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    return t
+from ._tensors import _need, _on_device, _ptr, _stream
+from .linear import linear_i8
 
 
 class LossLog:
@@ -781,6 +740,20 @@ class YOLOv1Head(nn.Module):
             else:
                 _lib.check(lib.yh_decode_nms_linear(out.data_ptr(), bias.data_ptr(), *tail, _stream(dev)))
         return (dets, count, kidx) if return_idx else (dets, count)
+
+    def postprocess_linear(self, x, layer, conf_thresh=0.5, iou_thresh=0.5, mode=_lib.YH_MODE_REFERENCE,
+                           return_idx=False):
+        """``postprocess`` of the last layer's output, from its input: ``x`` (B, K) features
+        (fp32, fp16 or bf16) go through ``layer``, an ``Int8Linear`` with S*S*D output channels
+        (model.py:133-135 in 8-bit integers), and its product and bias meet in the decode
+        kernel (model.py:146-148, 379-394).  Returns what ``postprocess`` returns."""
+        if x.dim() != 2:
+            raise ValueError(f"x: expected shape (B, K), got {tuple(x.shape)}")
+        if layer.out_features != self.depth * self.n_grid:
+            raise ValueError(f"layer: expected {self.depth * self.n_grid} output channels, got {layer.out_features}")
+        z = linear_i8(x, layer.weight, layer.weight_scale, out_dtype=torch.float32)
+        return self.postprocess(z.view(-1, self.depth, self.n_cells, self.n_cells), conf_thresh, iou_thresh, mode,
+                                return_idx, bias=layer.bias)
 
     @staticmethod
     def nms(ltrb, score, cls, present=None, conf_thresh=0.0, iou_thresh=0.5, return_idx=False):

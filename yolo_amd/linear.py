@@ -1,0 +1,153 @@
+"""The product of a linear layer in 8-bit integers, for serving the layers in front of the
+head (model.py:133-135): ``y = s_m t_n sum_k q_mk w_nk + bias_n`` with a scale for every row of
+the input (an image's features) and of the weight (an output channel).
+
+    layer = Int8Linear.from_linear(net[-1])               # weights quantised and laid out once
+    dets, count = head.postprocess_linear(features, layer)
+
+The sum is exact in int32; scales and bias are applied in fp32.  Forward only."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch import nn
+
+from . import _lib
+from ._tensors import _need, _on_device, _ptr, _stream
+
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _no_grad(t: torch.Tensor, name: str) -> None:
+    if torch.is_grad_enabled() and t.requires_grad:
+        raise ValueError(f"{name}: requires a gradient, and the 8-bit product has none; call it under "
+                         "torch.no_grad() or on a detached tensor")
+
+
+def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
+    """(..., K) as (M, K) with unit stride along K; a view where the strides allow one."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor, got {type(x).__name__}")
+    if not x.is_cuda:
+        raise ValueError(f"{name}: must live on the GPU (got device {x.device}); yolo_amd has no CPU path")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= _lib.YH_MAX_I8_K:
+        raise ValueError(f"{name}: expected shape (..., K) with K in 1 .. {_lib.YH_MAX_I8_K}, got {tuple(x.shape)}")
+    if x.stride(-1) != 1 and x.shape[-1] > 1:
+        raise ValueError(f"{name}: must be contiguous along its last axis")
+    x = x.detach()
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1]) if x.numel() else x.new_empty(0, x.shape[-1])
+    if x.shape[0] > 1 and x.stride(0) < x.shape[1]:      # expanded or overlapping rows
+        x = x.contiguous()
+    return x
+
+
+def _ld(x: torch.Tensor) -> int:
+    return x.stride(0) if x.shape[0] > 1 else max(x.stride(0), x.shape[1])
+
+
+def quantize_rows(x: torch.Tensor):
+    """``x`` (M, K) fp32, fp16 or bf16 -> ``(q, scale)``: ``scale[m] = max_k |x[m, k]| / 127`` (fp32) and
+    ``q[m, k] = 127 x[m, k] / max_k |x[m, k]|`` to the nearest whole number, ties to even, as int8.
+
+    ``q`` has shape (M, K); its rows lie a multiple of 128 bytes apart with zeros behind them, the
+    layout ``linear_i8`` takes for a weight.  A row of zeros gets scale 0; a row that holds a NaN or
+    an infinity gets scale NaN and zeros."""
+    _no_grad(x, "x")
+    if isinstance(x, torch.Tensor) and x.dim() != 2:
+        raise ValueError(f"x: expected shape (M, K), got {tuple(x.shape)}")
+    x = _rows(x, "x")
+    if x.dtype not in _FLOATS:
+        raise ValueError(f"x: expected dtype float32, float16 or bfloat16, got {x.dtype}")
+    m, k = x.shape
+    q = torch.empty(m, (k + 127) // 128 * 128, dtype=torch.int8, device=x.device)
+    scale = torch.empty(m, dtype=torch.float32, device=x.device)
+    with _on_device(x.device):
+        _lib.check(_lib.load().yh_quantize_rows(x.data_ptr(), _lib.DTYPE_CODES[x.dtype], _ld(x), q.data_ptr(), q.shape[1],
+                                                scale.data_ptr(), m, k, _stream(x.device)))
+    return q[:, :k], scale
+
+
+def linear_i8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+              x_scale: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``y[..., n] = s t_n sum_k q_k w_nk + bias_n``: ``x`` (..., K) times ``weight`` (N, K) int8 with ``weight_scale`` (N).
+
+    ``x`` is fp32, fp16 or bf16 and is quantised row by row as ``quantize_rows`` does, or int8 with the
+    scales of its rows in ``x_scale``.  ``weight`` as ``quantize_rows`` returns it: unit stride along K, rows a
+    multiple of 16 bytes apart.  ``bias`` (N) fp32.  The result has ``out_dtype`` (fp32, fp16, bf16; by
+    default that of ``x``, fp32 for an int8 ``x``)."""
+    _no_grad(x, "x")
+    shape = x.shape
+    x = _rows(x, "x")
+    m, k = x.shape
+    dev = x.device
+    if x.dtype not in _lib.DTYPE_CODES:
+        raise ValueError(f"x: expected dtype float32, float16, bfloat16 or int8, got {x.dtype}")
+    if (x.dtype == torch.int8) != (x_scale is not None):
+        raise ValueError("x_scale: the scales of an int8 x, and of nothing else")
+    if x_scale is not None:
+        _need(x_scale, "x_scale", torch.float32)
+        if x_scale.numel() != m:
+            raise ValueError(f"x_scale: expected {m} values, got {x_scale.numel()}")
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.shape[1] != k or weight.dtype != torch.int8:
+        raise ValueError(f"weight: expected an int8 tensor of shape (N, {k})")
+    n = weight.shape[0]
+    ldw = weight.stride(0) if n > 1 else (k + 15) // 16 * 16
+    end = weight.storage_offset() + (n - 1) * ldw + (k + 15) // 16 * 16
+    if n and ((weight.stride(1) != 1 and k > 1) or ldw < k or ldw % 16 or weight.data_ptr() % 16
+              or end > weight.untyped_storage().nbytes()):
+        raise ValueError("weight: unit stride along K, rows a multiple of 16 bytes apart and 16-byte aligned, the last one "
+                         "with room up to the next multiple of 16 bytes (quantize_rows lays it out so)")
+    _need(weight_scale, "weight_scale", torch.float32, (n,))
+    if bias is not None:
+        bias = _need(bias.detach(), "bias", torch.float32, (n,))
+    for name, t in (("weight", weight), ("weight_scale", weight_scale), ("bias", bias), ("x_scale", x_scale)):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name}: on {t.device}, x is on {dev}")
+    if out_dtype is None:
+        out_dtype = torch.float32 if x.dtype == torch.int8 else x.dtype
+    if out_dtype not in _FLOATS:
+        raise ValueError(f"out_dtype: expected float32, float16 or bfloat16, got {out_dtype}")
+    y = torch.empty(*shape[:-1], n, dtype=out_dtype, device=dev)
+    if y.numel() == 0:
+        return y
+    lib = _lib.load()
+    ws = torch.empty(lib.yh_linear_i8_workspace_bytes(m, n, k), dtype=torch.uint8, device=dev)
+    with _on_device(dev):
+        _lib.check(lib.yh_linear_i8(x.data_ptr(), _lib.DTYPE_CODES[x.dtype], _ld(x), _ptr(x_scale), weight.data_ptr(), ldw,
+                                    weight_scale.data_ptr(), _ptr(bias), y.data_ptr(), _lib.DTYPE_CODES[out_dtype], n, m, n,
+                                    k, ws.data_ptr(), ws.numel(), _stream(dev)))
+    return y
+
+
+class Int8Linear(nn.Module):
+    """A linear layer served in 8-bit integers: ``forward(x)`` is ``linear_i8`` with this layer's weight,
+    scales and bias.  The weight is quantised and laid out once, by ``from_linear``."""
+
+    def __init__(self, weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optional[torch.Tensor] = None):
+        super().__init__()
+        self.out_features, self.in_features = weight.shape
+        rows = weight.new_zeros(self.out_features, (self.in_features + 127) // 128 * 128)
+        rows[:, :self.in_features] = weight
+        self.register_buffer("weight_rows", rows)
+        self.register_buffer("weight_scale", weight_scale.detach().clone())
+        self.register_buffer("bias", None if bias is None else bias.detach().float().clone())
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear) -> "Int8Linear":
+        """The weight of ``linear`` (fp32, fp16 or bf16, on the GPU) with a scale for each output channel."""
+        with torch.no_grad():
+            q, scale = quantize_rows(linear.weight.detach().contiguous())
+            return cls(q, scale, linear.bias)
+
+    @property
+    def weight(self) -> torch.Tensor:
+        """(out_features, in_features) int8, rows a multiple of 128 bytes apart."""
+        return self.weight_rows[:, :self.in_features]
+
+    def forward(self, x: torch.Tensor, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        return linear_i8(x, self.weight, self.weight_scale, bias=self.bias, out_dtype=out_dtype)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"

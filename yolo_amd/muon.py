@@ -1,0 +1,167 @@
+"""Orthogonalised updates for weight matrices: ``orthogonalize`` (Newton-Schulz steps towards the nearest
+matrix with orthonormal rows), ``muon_step`` (momentum, orthogonalised update and weight step of
+matrices of one shape) and ``Muon``, the optimizer made of it, for the convolutions and linear layers in
+front of the head (the reference trains them with AdamW, train.py:84-94):
+
+    weights = [p for p in net.parameters() if p.dim() >= 2]
+    optim = Muon(weights, lr=0.02)
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Sequence, Tuple
+
+import torch
+
+from . import _lib
+from ._tensors import _need, _on_device, _stream
+
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+COEFFS = (3.4445, -4.7750, 2.0315)      # raises small singular values fastest; they end within 0.7 .. 1.2
+
+
+def _workspace(lib, count: int, rows: int, cols: int, device) -> torch.Tensor:
+    nbytes = lib.yh_orthogonalize_workspace_bytes(count, rows, cols)
+    if nbytes == 0:
+        raise ValueError(f"{count} matrices of {rows} x {cols}: outside the supported range (shorter side up to 32,768, "
+                         "longer up to 2^24)")
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def _check_steps(steps: int, eps: float) -> None:
+    if not 1 <= int(steps) <= _lib.YH_MAX_NS_STEPS:
+        raise ValueError(f"steps: expected 1 .. {_lib.YH_MAX_NS_STEPS}, got {steps}")
+    if not (eps >= 0 and math.isfinite(eps)):
+        raise ValueError(f"eps: expected a finite number that is not negative, got {eps}")
+
+
+def orthogonalize(g: torch.Tensor, steps: int = 5, coeffs: Tuple[float, float, float] = COEFFS, eps: float = 1e-7,
+                  out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``steps`` times ``X <- (a + b X X' + c (X X')^2) X`` from ``X = g / (|g| + eps)`` for every matrix of
+    ``g`` (..., rows, cols), fp32, fp16 or bf16; a matrix taller than wide is worked on transposed.
+
+    Columns lie next to each other and rows at any stride of at least ``cols``; leading axes collapse to one.
+    The matrices are held in 22 bits: the result (contiguous, ``out_dtype``) is about 1e-4 off the exact one
+    (3e-5 when it is fp32) before its rounding.  A NaN or an infinity makes its whole matrix NaN.  Forward only."""
+    if not isinstance(g, torch.Tensor):
+        raise TypeError(f"g: expected a torch.Tensor, got {type(g).__name__}")
+    if not g.is_cuda:
+        raise ValueError(f"g: must live on the GPU (got device {g.device}); yolo_amd has no CPU path")
+    if g.dtype not in _FLOATS or out_dtype not in _FLOATS:
+        raise ValueError(f"g and out_dtype: expected float32, float16 or bfloat16, got {g.dtype} and {out_dtype}")
+    if torch.is_grad_enabled() and g.requires_grad:
+        raise ValueError("g: requires a gradient, and orthogonalize has none; pass g.detach()")
+    if g.dim() < 2:
+        raise ValueError(f"g: expected shape (..., rows, cols), got {tuple(g.shape)}")
+    _check_steps(steps, eps)
+    out = torch.empty(g.shape, dtype=out_dtype, device=g.device)
+    if g.numel() == 0:
+        return out
+    rows, cols = g.shape[-2:]
+    if (cols > 1 and g.stride(-1) != 1) or (rows > 1 and g.stride(-2) < cols):
+        raise ValueError("g: columns must lie next to each other and rows at least a row apart (pass g.contiguous(); for a "
+                         "transposed matrix orthogonalize the original and transpose the result)")
+    batch = g.reshape(-1, rows, cols)
+    count = batch.shape[0]
+    lib = _lib.load()
+    ws = _workspace(lib, count, rows, cols, g.device)
+    ld = batch.stride(1) if rows > 1 else cols
+    with _on_device(g.device):
+        _lib.check(lib.yh_orthogonalize(
+            batch.data_ptr(), _lib.DTYPE_CODES[g.dtype], batch.stride(0) if count > 1 else rows * ld, ld, out.data_ptr(),
+            _lib.DTYPE_CODES[out_dtype], rows * cols, cols, count, rows, cols, *(float(v) for v in coeffs), int(steps),
+            float(eps), ws.data_ptr(), ws.numel(), _stream(g.device)))
+    return out
+
+
+def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], momenta: Sequence[torch.Tensor], lr: float,
+              momentum: float = 0.95, weight_decay: float = 0.0, nesterov: bool = True, scale: Optional[float] = None,
+              steps: int = 5, coeffs: Tuple[float, float, float] = COEFFS, eps: float = 1e-7) -> None:
+    """One step of weights of one shape, in place: ``m <- momentum m + g``; ``u = g + momentum m`` (``nesterov``)
+    or ``m``; ``p <- (1 - lr weight_decay) p - lr scale orthogonalize(u)``.
+
+    ``params`` (fp32, fp16 or bf16), ``grads`` (fp32, fp16 or bf16) and ``momenta`` (fp32) are sequences of
+    contiguous tensors of one shape each; an axis beyond the second is folded into the columns (a
+    convolution's cout x cin*k*k).  ``scale`` defaults to ``sqrt(max(1, rows / cols))``.  A captured graph replays
+    the step with the tensors and numbers it was captured with."""
+    if not (len(params) == len(grads) == len(momenta)):
+        raise ValueError(f"{len(params)} params, {len(grads)} grads and {len(momenta)} momenta")
+    if not params:
+        return
+    first = params[0]
+    shape, dev = tuple(first.shape), first.device
+    if len(shape) < 2:
+        raise ValueError(f"params: expected at least two axes, got {shape}")
+    if first.dtype not in _FLOATS or grads[0].dtype not in _FLOATS:
+        raise ValueError(f"params and grads: expected float32, float16 or bfloat16, got {first.dtype} and {grads[0].dtype}")
+    for name, tensors, dtype in (("params", params, first.dtype), ("grads", grads, grads[0].dtype),
+                                 ("momenta", momenta, torch.float32)):
+        for i, t in enumerate(tensors):
+            _need(t.detach(), f"{name}[{i}]", dtype, shape)
+            if t.device != dev:
+                raise ValueError(f"{name}[{i}]: on {t.device}, params[0] is on {dev}")
+    _check_steps(steps, eps)
+    if first.numel() == 0:
+        return
+    spans = sorted([(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), 1) for t in (*params, *momenta)]
+                   + [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), 0) for t in grads])
+    end, end_written = 0, 0
+    for lo, hi, written in spans:        # what is written overlaps nothing; a gradient may serve two weights
+        if lo < end_written or (written and lo < end):
+            raise ValueError("params and momenta: each in memory of its own; the same memory is given twice")
+        end, end_written = max(end, hi), max(end_written, hi if written else 0)
+    rows, cols = shape[0], first.numel() // shape[0]
+    if scale is None:
+        scale = math.sqrt(max(1.0, rows / cols))
+    lib = _lib.load()
+    most = _lib.YH_MUON_MAX_COUNT
+    for at in range(0, len(params), most):
+        some = slice(at, at + most)
+        count = len(params[some])
+        ws = _workspace(lib, count, rows, cols, dev)
+        lists = [(ctypes.c_void_p * count)(*(t.data_ptr() for t in tensors[some])) for tensors in (params, grads, momenta)]
+        with _on_device(dev):
+            _lib.check(lib.yh_muon_step(
+                lists[0], _lib.DTYPE_CODES[first.dtype], lists[1], _lib.DTYPE_CODES[grads[0].dtype], lists[2], count, rows, cols,
+                float(lr), float(momentum), int(bool(nesterov)), float(weight_decay), float(scale), *(float(v) for v in coeffs),
+                int(steps), float(eps), ws.data_ptr(), ws.numel(), _stream(dev)))
+    for t in (*params, *momenta):
+        torch.autograd.graph.increment_version(t)
+
+
+class Muon(torch.optim.Optimizer):
+    """``muon_step`` as an optimizer over weights of two or more axes (convolutions, linear layers); biases and
+    norms belong to another optimizer.  Weights of one shape and type are stepped together."""
+
+    def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, weight_decay: float = 0.0, nesterov: bool = True,
+                 steps: int = 5, coeffs: Tuple[float, float, float] = COEFFS, eps: float = 1e-7):
+        _check_steps(steps, eps)
+        super().__init__(params, dict(lr=lr, momentum=momentum, weight_decay=weight_decay, nesterov=nesterov, steps=steps,
+                                      coeffs=tuple(coeffs), eps=eps))
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.dim() < 2:
+                    raise ValueError(f"Muon: a parameter of shape {tuple(p.shape)}; weights of two or more axes only")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            alike = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                state = self.state[p]
+                if "momentum_buffer" not in state:
+                    state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                alike.setdefault((tuple(p.shape), p.dtype, p.grad.dtype, p.device), []).append(p)
+            for ps in alike.values():
+                muon_step(ps, [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p in ps],
+                          [self.state[p]["momentum_buffer"] for p in ps], lr=group["lr"], momentum=group["momentum"],
+                          weight_decay=group["weight_decay"], nesterov=group["nesterov"], steps=group["steps"],
+                          coeffs=group["coeffs"], eps=group["eps"])
+        return loss
