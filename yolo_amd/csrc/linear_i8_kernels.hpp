@@ -174,10 +174,10 @@ __device__ __forceinline__ void linear_store(const LinearI8Args& a, long long m,
     put4<DT>((typename Elem<DT>::T*)a.y + m * a.ldy + n, v, left, a.whole);
 }
 
-template <int DT, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void linear_i8_tile_kernel(LinearI8Args a) {
-    typedef TileProduct<MathI8, BM, BN, WM, WN, true> P;
-    extern __shared__ __align__(16) char lds[];
+template <int DT, int BM, int BN, int WM, int WN, int STAGES>
+__global__ __launch_bounds__(64 * WM * WN, 2) void linear_i8_tile_kernel(LinearI8Args a) {
+    typedef TileProduct<MathI8, BM, BN, WM, WN, STAGES, true> P;
+    YH_TILE_RING(P)
     const long long tiles = (long long)a.tiles_m * a.tiles_n;
     const long long id = xcd_order(blockIdx.x, tiles * a.slices);
     const int slice = (int)(id / tiles);
@@ -190,9 +190,9 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_i8_tile_kernel(LinearI8Ar
     typename P::Acc acc[P::TM][P::TN] = {};
     const TileOperand A = {(const char*)a.q, a.ldq, a.M, tm * BM, (long long)a.blocks * 128 - 16};
     const TileOperand B = {(const char*)a.w, a.ldw, a.N, tn * BN, a.last_w};
-    const long long k0 = (long long)slice * a.per_slice;
-    const long long k1 = k0 + a.per_slice < a.blocks ? k0 + a.per_slice : a.blocks;
-    P::run(A, B, k0, k1, lds, acc);
+    const int k0 = slice * a.per_slice;
+    const int k1 = k0 + a.per_slice < a.blocks ? k0 + a.per_slice : a.blocks;
+    P::run(A, B, k0, k1, ring, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long long m0 = tm * BM + (wave / WN) * (BM / WM) + piece_across(lane);
     const long long n0 = tn * BN + (wave % WN) * (BN / WN) + piece_along(lane);

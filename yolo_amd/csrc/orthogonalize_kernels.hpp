@@ -218,10 +218,10 @@ __device__ __forceinline__ void ns_store_sym(const NsProduct& p, const NsProduct
     }
 }
 
-template <int BM, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void ns_product_kernel(NsProducts a) {
-    typedef TileProduct<MathSplit, BM, BM, WM, WN, true> T;
-    extern __shared__ __align__(16) char lds[];
+template <int BM, int WM, int WN, int STAGES>
+__global__ __launch_bounds__(64 * WM * WN, 2) void ns_product_kernel(NsProducts a) {
+    typedef TileProduct<MathSplit, BM, BM, WM, WN, STAGES, true> T;
+    YH_TILE_RING(T)
     const NsProduct p = a.job[blockIdx.y];
     const long long per = (long long)a.tiles * a.count;
     const long long id = xcd_order(blockIdx.x, per * a.slices);
@@ -233,9 +233,9 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_product_kernel(NsProducts a) 
     typename T::Acc acc[T::TM][T::TN] = {};
     const TileOperand A = {p.P + mat * p.p_mat, p.ldp, a.l, (long long)ti * BM, p.ldp - 16};
     const TileOperand B = {p.Q + mat * p.p_mat, p.ldp, a.l, (long long)tj * BM, p.ldp - 16};
-    const long long k0 = (long long)slice * a.per_slice;
-    const long long k1 = k0 + a.per_slice < p.blocks ? k0 + a.per_slice : p.blocks;
-    T::run(A, B, k0, k1, lds, acc);
+    const int k0 = slice * a.per_slice;
+    const int k1 = k0 + a.per_slice < p.blocks ? k0 + a.per_slice : p.blocks;
+    T::run(A, B, k0, k1, ring, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long long m0 = (long long)ti * BM + (wave / WN) * (BM / WM) + piece_across(lane);
     const long long n0 = (long long)tj * BM + (wave % WN) * (BM / WN) + piece_along(lane);
@@ -250,9 +250,9 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_product_kernel(NsProducts a) 
 }
 
 // the slices of ns_product_kernel added in order, same geometry
-template <int BM, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void ns_join_kernel(NsProducts a) {
-    typedef TileProduct<MathSplit, BM, BM, WM, WN, true> T;
+template <int BM, int WM, int WN, int STAGES>
+__global__ __launch_bounds__(64 * WM * WN, 2) void ns_join_kernel(NsProducts a) {
+    typedef TileProduct<MathSplit, BM, BM, WM, WN, STAGES, true> T;
     const NsProduct p = a.job[0];
     const long long per = (long long)a.tiles * a.count;
     const long long mt = blockIdx.x;
@@ -294,12 +294,12 @@ struct NsApply {
     float again;
 };
 
-template <int DT, int OUT, bool TALL, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void ns_apply_kernel(NsApply a) {
+template <int DT, int OUT, bool TALL, int BM, int BN, int WM, int WN, int STAGES>
+__global__ __launch_bounds__(64 * WM * WN, 2) void ns_apply_kernel(NsApply a) {
     // a lane's four numbers lie along a row of the result: along n, or along l when X is G'
-    typedef TileProduct<MathSplit, BM, BN, WM, WN, !TALL> T;
+    typedef TileProduct<MathSplit, BM, BN, WM, WN, STAGES, !TALL> T;
     typedef typename Elem<DT>::T E;
-    extern __shared__ __align__(16) char lds[];
+    YH_TILE_RING(T)
     const NsShape& sh = a.sh;
     const int tl = (int)((sh.l + BM - 1) / BM);
     const long long tn = (sh.n + BN - 1) / BN, per = tl * tn;
@@ -310,7 +310,7 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_apply_kernel(NsApply a) {
     const long long ld = sh.lk * 4, ldn = sh.nk * 4;
     const TileOperand A = {a.S + mat * a.s_mat, ld, sh.l, ti * BM, ld - 16};
     const TileOperand B = {a.Xt + mat * a.xt_mat, ld, sh.n, tj * BN, ld - 16};
-    T::run(A, B, 0, sh.lk / 32, lds, acc);
+    T::run(A, B, 0, (int)(sh.lk / 32), ring, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const char* x = TALL ? a.Xt + mat * a.xt_mat : a.X + mat * a.x_mat;
     const long long ldx = TALL ? ld : ldn;

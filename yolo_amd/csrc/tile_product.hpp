@@ -27,21 +27,36 @@ typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 
 struct MathI8 {
     using Acc = v4i;
-    static __device__ __forceinline__ void mma(Acc& d, const v4i (&p)[2], const v4i (&q)[2]) {
-        d = __builtin_amdgcn_mfma_i32_16x16x64_i8(p[0], q[0], d, 0, 0, 0);
-        d = __builtin_amdgcn_mfma_i32_16x16x64_i8(p[1], q[1], d, 0, 0, 0);
+    static constexpr int PASSES = 2;
+    template <int PASS> static __device__ __forceinline__ void mma(Acc& d, const v4i (&p)[2], const v4i (&q)[2]) {
+        d = __builtin_amdgcn_mfma_i32_16x16x64_i8(p[PASS], q[PASS], d, 0, 0, 0);
     }
 };
 
 struct MathSplit {
     using Acc = v4f;
-    static __device__ __forceinline__ v8h h(v4i x) { return __builtin_bit_cast(v8h, x); }
-    static __device__ __forceinline__ void mma(Acc& d, const v4i (&p)[2], const v4i (&q)[2]) {
-        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(h(p[0]), h(q[1]), d, 0, 0, 0);
-        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(h(p[1]), h(q[0]), d, 0, 0, 0);
-        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(h(p[0]), h(q[0]), d, 0, 0, 0);
+    static constexpr int PASSES = 3;
+    // lo * hi, hi * lo, then hi * hi
+    template <int PASS> static __device__ __forceinline__ void mma(Acc& d, const v4i (&p)[2], const v4i (&q)[2]) {
+        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, p[PASS == 0]), __builtin_bit_cast(v8h, q[PASS == 1]), d,
+                                                   0, 0, 0);
     }
 };
+
+// acc[j] += fragment a * fragment b[j] (or the other way round), pass by pass: consecutive instructions write
+// different registers
+template <class Math, bool ROWS_B, int PASS, int TN>
+__device__ __forceinline__ void mma_row(typename Math::Acc (&acc)[TN], const v4i (&fa)[2], const v4i (&fb)[TN][2]) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+        if (ROWS_B) Math::template mma<PASS>(acc[j], fb[j], fa);
+        else Math::template mma<PASS>(acc[j], fa, fb[j]);
+    }
+    if constexpr (PASS + 1 < Math::PASSES) mma_row<Math, ROWS_B, PASS + 1, TN>(acc, fa, fb);
+}
+
+typedef __attribute__((address_space(3))) char* LdsPtr;
+typedef const __attribute__((address_space(3))) v4i* LdsFragment;
 
 constexpr int TILE_BLOCK_BYTES = 128;   // of a row, per step of the contraction
 
@@ -53,98 +68,117 @@ struct TileOperand {
     long long ld;           // bytes from row to row
     long long rows;
     long long first;
-    long long last_chunk;
+    long long last_chunk;   // below 2^31
 };
 
 // A workgroup of WM x WN wavefronts computes BM x BN numbers over the blocks [kb0, kb1) of the contraction.
 // acc[i][j] of a wavefront is the 16x16 piece (i, j) of its BM/WM x BN/WN part.  Rows of D (register index) run
 // along B when ROWS_B, along A otherwise: the caller picks what its stores want contiguous in a lane.
-// lds: 2 * (BM + BN) * 128 bytes.  The next block's bytes travel in registers while a block is worked on
-// (double-buffered LDS, one barrier per block).
-template <class Math, int BM, int BN, int WM, int WN, bool ROWS_B>
+//
+// A ring of STAGES blocks in LDS: while one is worked on, the next STAGES - 1 are on their way, straight from memory into
+// LDS (16 bytes a lane, no registers in between; the exchange of chunks is made in the address a lane reads, since a
+// wavefront's 1,024 bytes land in LDS in lane order).  A load takes about 1 us, a block's products 0.2 us (128 x 128) to
+// 0.9 us (256 x 256): what is in flight hides the difference, within a workgroup by stages and on a CU by several
+// workgroups.  The stages are distinct objects, so reads of one need not wait for loads into another.  One barrier per
+// block: it says that the block has landed for every wavefront and that the block before it has been read by all.
+template <class Math, int BM, int BN, int WM, int WN, int STAGES, bool ROWS_B>
 struct TileProduct {
-    static constexpr int THREADS = 64 * WM * WN;
+    static constexpr int THREADS = 64 * WM * WN, DEPTH = STAGES;
     static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
-    static constexpr int LDS_BYTES = 2 * (BM + BN) * TILE_BLOCK_BYTES;
-    static constexpr int LA = BM * 8 / THREADS, LB = BN * 8 / THREADS;   // 16-byte loads per thread
+    static constexpr int HALF = (BM + BN) * TILE_BLOCK_BYTES;
+    static constexpr int WAVES = WM * WN;
+    static constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;   // 1,024-byte loads (8 rows) of a wavefront per block
+    static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "whole loads");
+    static_assert(STAGES >= 2 && STAGES <= 4, "a ring of two to four");
     using Acc = typename Math::Acc;
 
-    static __device__ __forceinline__ void run(const TileOperand& A, const TileOperand& B, long long kb0, long long kb1,
-                                               char* lds, Acc (&acc)[TM][TN]) {
-        const int t = threadIdx.x, chunk = t & 7, row0 = t >> 3;
-        constexpr int STEP = THREADS / 8;
-        const char* pa[LA];
-        const char* pb[LB];
+    static __device__ __forceinline__ void block(LdsPtr s, int abase, int bbase, int c0, int c1, Acc (&acc)[TM][TN]) {
+        v4i fb[TN][2];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            fb[j][0] = *(LdsFragment)(s + bbase + j * 16 * TILE_BLOCK_BYTES + c0);
+            fb[j][1] = *(LdsFragment)(s + bbase + j * 16 * TILE_BLOCK_BYTES + c1);
+        }
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            v4i fa[2];
+            fa[0] = *(LdsFragment)(s + abase + i * 16 * TILE_BLOCK_BYTES + c0);
+            fa[1] = *(LdsFragment)(s + abase + i * 16 * TILE_BLOCK_BYTES + c1);
+            mma_row<Math, ROWS_B, 0, TN>(acc[i], fa, fb);
+        }
+    }
+
+    // all but the N youngest loads of this wavefront have landed and its LDS reads are done; then every wavefront's
+    template <int N> static __device__ __forceinline__ void landed() {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);      // vmcnt(N) lgkmcnt(0), expcnt as it is
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    }
+
+    static __device__ __forceinline__ void run(const TileOperand& A, const TileOperand& B, int kb0, int kb1, const LdsPtr (&ring)[4],
+                                               Acc (&acc)[TM][TN]) {
+        const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+        const int group = __builtin_amdgcn_readfirstlane(wave) * 8;       // of 8 rows, every WAVES-th is this wavefront's
+        const int row = group + (lane >> 3);
+        const int chunk = ((lane & 7) ^ (lane >> 3)) << 4;
+        const int last_a = (int)A.last_chunk, last_b = (int)B.last_chunk;
+        const char *pa[LA], *pb[LB];
 #pragma unroll
         for (int i = 0; i < LA; ++i) {
-            const long long r = A.first + row0 + i * STEP;
+            const long long r = A.first + row + i * 8 * WAVES;
             pa[i] = A.base + (r < A.rows ? r : A.rows - 1) * A.ld;
         }
 #pragma unroll
         for (int i = 0; i < LB; ++i) {
-            const long long r = B.first + row0 + i * STEP;
+            const long long r = B.first + row + i * 8 * WAVES;
             pb[i] = B.base + (r < B.rows ? r : B.rows - 1) * B.ld;
         }
-        v4i ra[LA], rb[LB];
-        auto fetch = [&](long long kb) {
-            const long long off = kb * TILE_BLOCK_BYTES + chunk * 16;
-            const long long oa = off < A.last_chunk ? off : A.last_chunk, ob = off < B.last_chunk ? off : B.last_chunk;
-#pragma unroll
-            for (int i = 0; i < LA; ++i) ra[i] = *(const v4i*)(pa[i] + oa);
-#pragma unroll
-            for (int i = 0; i < LB; ++i) rb[i] = *(const v4i*)(pb[i] + ob);
+        auto to_lds = [](const char* from, LdsPtr to) {
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                             (__attribute__((address_space(3))) void*)to, 16, 0, 0);
         };
-        auto park = [&](char* s) {
+        auto load = [&](LdsPtr s, int kb) {
+            const int off = kb * TILE_BLOCK_BYTES + chunk;
+            const int oa = off < last_a ? off : last_a, ob = off < last_b ? off : last_b;
 #pragma unroll
-            for (int i = 0; i < LA; ++i) {
-                const int r = row0 + i * STEP;
-                *(v4i*)(s + r * TILE_BLOCK_BYTES + ((chunk ^ (r & 7)) << 4)) = ra[i];
-            }
+            for (int i = 0; i < LA; ++i) to_lds(pa[i] + oa, s + (group + i * 8 * WAVES) * TILE_BLOCK_BYTES);
 #pragma unroll
-            for (int i = 0; i < LB; ++i) {
-                const int r = row0 + i * STEP;
-                *(v4i*)(s + (BM + r) * TILE_BLOCK_BYTES + ((chunk ^ (r & 7)) << 4)) = rb[i];
-            }
+            for (int i = 0; i < LB; ++i) to_lds(pb[i] + ob, s + (BM + group + i * 8 * WAVES) * TILE_BLOCK_BYTES);
         };
-        const int lane = t & 63, wave = t >> 6;
         const int wm = wave / WN, wn = wave % WN;
         const int lr = lane & 15, lq = lane >> 4;
         const int c0 = (lq ^ (lr & 7)) << 4, c1 = ((4 + lq) ^ (lr & 7)) << 4;
         const int abase = (wm * (BM / WM) + lr) * TILE_BLOCK_BYTES;
         const int bbase = (BM + wn * (BN / WN) + lr) * TILE_BLOCK_BYTES;
-        constexpr int HALF = (BM + BN) * TILE_BLOCK_BYTES;
         if (kb0 >= kb1) return;
-        fetch(kb0);
-        park(lds);
-        __syncthreads();
-        int cur = 0;
-        for (long long kb = kb0; kb < kb1; ++kb) {
-            const bool more = kb + 1 < kb1;
-            if (more) fetch(kb + 1);
-            const char* s = lds + cur * HALF;
-            v4i fb[TN][2];
+        // Loads past the last block bring it in once more and are not used: every load of the loop is issued, so what is on
+        // its way at any point is known when this is compiled (a load behind a branch makes the compiler wait for all).
+        const int end = kb1 - 1;
 #pragma unroll
-            for (int j = 0; j < TN; ++j) {
-                fb[j][0] = *(const v4i*)(s + bbase + j * 16 * TILE_BLOCK_BYTES + c0);
-                fb[j][1] = *(const v4i*)(s + bbase + j * 16 * TILE_BLOCK_BYTES + c1);
+        for (int u = 0; u < STAGES - 1; ++u) load(ring[u], kb0 + u < end ? kb0 + u : end);
+        int kb = kb0;
+        for (; kb + STAGES <= kb1; kb += STAGES) {
+#pragma unroll
+            for (int u = 0; u < STAGES; ++u) {
+                landed<(STAGES - 2) * (LA + LB)>();       // this block; STAGES - 2 more are behind it
+                const int next = kb + u + STAGES - 1;
+                load(ring[(u + STAGES - 1) % STAGES], next < end ? next : end);
+                block(ring[u], abase, bbase, c0, c1, acc);
             }
-#pragma unroll
-            for (int i = 0; i < TM; ++i) {
-                v4i fa[2];
-                fa[0] = *(const v4i*)(s + abase + i * 16 * TILE_BLOCK_BYTES + c0);
-                fa[1] = *(const v4i*)(s + abase + i * 16 * TILE_BLOCK_BYTES + c1);
-#pragma unroll
-                for (int j = 0; j < TN; ++j) {
-                    if (ROWS_B) Math::mma(acc[i][j], fb[j], fa);
-                    else Math::mma(acc[i][j], fa, fb[j]);
-                }
-            }
-            if (more) park(lds + (cur ^ 1) * HALF);
-            __syncthreads();
-            cur ^= 1;
         }
+        landed<0>();
+#pragma unroll
+        for (int u = 0; u < STAGES - 1; ++u)
+            if (kb + u < kb1) block(ring[u], abase, bbase, c0, c1, acc);
     }
 };
+
+// the ring of a kernel whose TileProduct is T (up to four stages)
+#define YH_TILE_RING(T)                                                                                              \
+    __shared__ __align__(1024) char ring0[T::HALF], ring1[T::HALF], ring2[T::DEPTH > 2 ? T::HALF : 16],              \
+        ring3[T::DEPTH > 3 ? T::HALF : 16];                                                                          \
+    const LdsPtr ring[4] = {(LdsPtr)ring0, (LdsPtr)ring1, (LdsPtr)ring2, (LdsPtr)ring3};
 
 // Where a lane's four numbers of piece (i, j) lie in the tile: `along` is the first of the four consecutive
 // indices on the operand that supplies D's rows, `across` the index on the other one.

@@ -41,23 +41,52 @@ int quantize(const void* x, int dt, int64_t ldx, int8_t* q, int64_t ldq, float* 
     return launch_status();
 }
 
-// How the product is cut: tiles of BM x BN and slices of the contraction
+// How the product is cut: tiles of one of three sizes, and slices of the contraction.
+//
+//   tile      wavefronts  stages  LDS     block, one workgroup a CU / as many as fit (measured, us)
+//   128x256   8           3       144 KB  1.27
+//   128x128   8           4       128 KB  0.63
+//   64x64     4           3        48 KB  0.40 / 0.61 (three)
+//
+// A larger tile reads less per product (a CU takes in about 64 bytes a cycle), a smaller one fills the card when
+// there are few rows or channels.  The choice is the least time of: rounds of workgroups over the 256 CUs, times the
+// blocks of a slice (+ 3 us to start and end), plus, when the sums are joined, a launch and the traffic of the partial
+// sums.  One image never comes here (linear_i8_rows_kernel).
+struct Tile {
+    int bm, bn, per_cu;
+    double alone, shared;
+};
+constexpr Tile kTiles[3] = {{128, 256, 1, 1.27, 1.27}, {128, 128, 1, 0.63, 0.63}, {64, 64, 3, 0.40, 0.61}};
+
 struct Plan {
-    int tiles_m, tiles_n, slices, per_slice, blocks;
+    int tile, tiles_m, tiles_n, slices, per_slice, blocks;
     size_t q_off, s_off, p_off, total;
 };
 
 Plan plan_for(int64_t M, int64_t N, int64_t K) {
     Plan p = {};
     p.blocks = (int)((K + 127) / 128);
-    p.tiles_m = (int)((M + 127) / 128);
-    p.tiles_n = (int)((N + 127) / 128);
-    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-    int64_t s = tiles >= 256 ? 1 : (512 + tiles - 1) / tiles;
-    if (s > (p.blocks + 3) / 4) s = (p.blocks + 3) / 4;
-    if (s < 1) s = 1;
-    p.per_slice = (int)((p.blocks + s - 1) / s);
-    p.slices = (p.blocks + p.per_slice - 1) / p.per_slice;
+    double best = 0.0;
+    for (int t = 0; t < 3; ++t) {
+        const Tile& c = kTiles[t];
+        const int64_t tm = (M + c.bm - 1) / c.bm, tn = (N + c.bn - 1) / c.bn, tiles = tm * tn;
+        for (int s = 1; s <= 16 && s <= p.blocks; s *= 2) {
+            if (s > 1 && tiles * s > 2048) break;
+            const int64_t wgs = tiles * s, at_once = 256 * (int64_t)c.per_cu;
+            const int per = (p.blocks + s - 1) / s;
+            const double block = wgs <= 256 ? c.alone : c.shared;
+            double us = (double)((wgs + at_once - 1) / at_once) * (per * block + 3.0);
+            if (s > 1) us += 3.0 + (double)(s + 1) * (double)M * (double)N * 4.0 / 4e6;
+            if (best == 0.0 || us < best) {
+                best = us;
+                p.tile = t;
+                p.tiles_m = (int)tm;
+                p.tiles_n = (int)tn;
+                p.per_slice = per;
+                p.slices = (p.blocks + per - 1) / per;
+            }
+        }
+    }
     p.q_off = 0;
     p.s_off = up256((size_t)M * p.blocks * 128);
     p.p_off = p.s_off + up256((size_t)M * 4);
@@ -65,11 +94,17 @@ Plan plan_for(int64_t M, int64_t N, int64_t K) {
     return p;
 }
 
-template <int DT>
-int product(const LinearI8Args& a, hipStream_t st) {
-    typedef TileProduct<MathI8, 128, 128, 2, 2, true> P;
+template <int DT, int BM, int BN, int WM, int WN, int STAGES>
+void tiles(const LinearI8Args& a, hipStream_t st) {
     const unsigned grid = (unsigned)((int64_t)a.tiles_m * a.tiles_n * a.slices);
-    hipLaunchKernelGGL((linear_i8_tile_kernel<DT, 128, 128, 2, 2>), dim3(grid), dim3(P::THREADS), P::LDS_BYTES, st, a);
+    hipLaunchKernelGGL((linear_i8_tile_kernel<DT, BM, BN, WM, WN, STAGES>), dim3(grid), dim3(64 * WM * WN), 0, st, a);
+}
+
+template <int DT>
+int product(int tile, const LinearI8Args& a, hipStream_t st) {
+    if (tile == 0) tiles<DT, 128, 256, 2, 4, 3>(a, st);
+    else if (tile == 1) tiles<DT, 128, 128, 2, 4, 4>(a, st);
+    else tiles<DT, 64, 64, 2, 2, 3>(a, st);
     if (const int rc = launch_status()) return rc;
     if (a.slices > 1) {
         int64_t b = (a.M * ((a.N + 3) / 4) + 255) / 256;
@@ -81,7 +116,7 @@ int product(const LinearI8Args& a, hipStream_t st) {
 
 int check_sizes(int64_t M, int64_t N, int64_t K) {
     if (M < 0 || N < 0 || K < 1 || K > YH_MAX_I8_K || M > kMaxRows || N > kMaxRows) return YH_ERR_SHAPE;
-    if (((M + 127) / 128) * ((N + 127) / 128) >= ((int64_t)1 << 24)) return YH_ERR_SHAPE;
+    if (((M + 63) / 64) * ((N + 63) / 64) >= ((int64_t)1 << 22)) return YH_ERR_SHAPE;      // 512 threads a tile
     return YH_OK;
 }
 
@@ -157,9 +192,9 @@ int yh_linear_i8(const void* x, int x_dtype, int64_t ldx, const float* x_scale, 
     a.tiles_m = p.tiles_m;
     a.tiles_n = p.tiles_n;
     a.whole = (ldy * dtype_bytes(y_dtype)) % (4 * dtype_bytes(y_dtype)) == 0 && aligned(y, 4 * dtype_bytes(y_dtype));
-    if (y_dtype == YH_F32) return product<DT_F32>(a, st);
-    if (y_dtype == YH_F16) return product<DT_F16>(a, st);
-    return product<DT_BF16>(a, st);
+    if (y_dtype == YH_F32) return product<DT_F32>(p.tile, a, st);
+    if (y_dtype == YH_F16) return product<DT_F16>(p.tile, a, st);
+    return product<DT_BF16>(p.tile, a, st);
 }
 
 }  // extern "C"

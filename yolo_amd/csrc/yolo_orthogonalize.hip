@@ -20,7 +20,7 @@ inline size_t dtype_bytes(int dt) { return dt == YH_F32 ? 4 : 2; }
 
 constexpr int64_t kMaxShort = 32768, kMaxLong = (int64_t)1 << 24, kMaxNumbers = (int64_t)1 << 38;
 constexpr int TB = 128;                       // tile of the products
-typedef TileProduct<MathSplit, TB, TB, 2, 2, true> Tile;
+typedef TileProduct<MathSplit, TB, TB, 2, 4, 4, true> Tile;
 
 // powers of two the split matrices are held at: A and T up to about 1.5, R up to 127, S up to 1023
 constexpr float kScaleA = 512.0f, kScaleR = 512.0f, kScaleS = 64.0f, kScaleX = 4096.0f;
@@ -98,8 +98,8 @@ struct Sink {
 template <int DT, int OUT, bool TALL>
 int apply(const NsApply& a, hipStream_t st) {
     const int64_t tiles = ((a.sh.l + TB - 1) / TB) * ((a.sh.n + TB - 1) / TB) * a.sh.count;
-    hipLaunchKernelGGL((ns_apply_kernel<DT, OUT, TALL, TB, TB, 2, 2>), dim3((unsigned)tiles), dim3(Tile::THREADS),
-                       Tile::LDS_BYTES, st, a);
+    hipLaunchKernelGGL((ns_apply_kernel<DT, OUT, TALL, TB, TB, 2, 4, 4>), dim3((unsigned)tiles), dim3(Tile::THREADS),
+                       0, st, a);
     return launch_status();
 }
 
@@ -112,10 +112,10 @@ int apply_as(int dt, bool tall, const NsApply& a, hipStream_t st) {
 
 int products(const NsProducts& a, int jobs, hipStream_t st) {
     const unsigned grid = (unsigned)((int64_t)a.tiles * a.count * a.slices);
-    hipLaunchKernelGGL((ns_product_kernel<TB, 2, 2>), dim3(grid, (unsigned)jobs), dim3(Tile::THREADS), Tile::LDS_BYTES, st, a);
+    hipLaunchKernelGGL((ns_product_kernel<TB, 2, 4, 4>), dim3(grid, (unsigned)jobs), dim3(Tile::THREADS), 0, st, a);
     if (const int rc = launch_status()) return rc;
     if (a.slices > 1)
-        hipLaunchKernelGGL((ns_join_kernel<TB, 2, 2>), dim3((unsigned)(a.tiles * a.count)), dim3(Tile::THREADS), 0, st, a);
+        hipLaunchKernelGGL((ns_join_kernel<TB, 2, 4, 4>), dim3((unsigned)(a.tiles * a.count)), dim3(Tile::THREADS), 0, st, a);
     return launch_status();
 }
 
