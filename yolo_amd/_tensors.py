@@ -12,7 +12,10 @@ def _ptr(t: Optional[torch.Tensor]):
 
 
 def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The handle of the current stream of ``device`` (torch.cuda.current_stream builds an object around
+    it, which costs several microseconds per call)."""
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 class _on_device:

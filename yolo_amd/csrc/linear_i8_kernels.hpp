@@ -68,66 +68,170 @@ __device__ __forceinline__ int quantize_one(float x, double inv) {
     return (int)__builtin_rint(t);
 }
 
-// One workgroup per row; VEC: 16-byte loads (ldx and x allow them).  The row is read twice, the second time out
-// of L2.  A row that holds a NaN or an infinity gets the scale NaN and zeros, so every y of it is NaN.
-// Zeros are written from K to Kz (the padding the product's blocks of 128 bytes read).
-template <int DT, int THREADS>
-__global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const typename Elem<DT>::T* __restrict__ x,
-                                                                long long ldx, int8_t* __restrict__ q, long long ldq,
-                                                                float* __restrict__ scale, int K, int Kz, int vec) {
+// |x| as an integer orders as the number does, with infinities and NaNs above all numbers
+__device__ __forceinline__ unsigned magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// N numbers: x * inv in fp32 is off by at most 127 * 2^-23, so its nearest whole number is the right one unless it lies
+// that close to the middle of two; then (one group of 16 in a thousand, and where numbers are halves of the
+// largest) the group is done again in 64 bits.  Three times fewer cycles than 64 bits throughout.
+template <int N>
+__device__ __forceinline__ void quantize_some(const float (&x)[N], double inv, int8_t (&q)[N]) {
+    const float f = (float)inv;
+    bool near = false;
+    float r[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const float t = x[e] * f;
+        r[e] = __builtin_rintf(t);
+        near |= fabsf(t - r[e]) > 0.4999f;
+    }
+    // inv outside fp32's normal range (rows of tiny numbers) goes the exact way too
+    if (near || !(f > 1e-37f && f < 1e37f)) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) r[e] = (float)quantize_one(x[e], inv);
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) q[e] = (int8_t)(int)r[e];
+}
+
+// 16 numbers of a row from i on, zeros past K; vec: the row lies on 16 bytes
+template <int DT>
+__device__ __forceinline__ void load16(const typename Elem<DT>::T* row, int i, int K, bool vec, float (&f)[16]) {
     typedef typename Elem<DT>::T T;
     constexpr int V = 16 / (int)sizeof(T);
     typedef T TV __attribute__((ext_vector_type(V)));
-    const T* row = x + (long long)blockIdx.x * ldx;
-    int8_t* out = q + (long long)blockIdx.x * ldq;
-    const int t = threadIdx.x;
-    __shared__ unsigned part[THREADS / 64];
-    // |x| as an integer orders as the number does, with infinities and NaNs above all numbers
-    unsigned top = 0;
-    if (vec) {
-        const int nv = K / V;
-        for (int i = t; i < nv; i += THREADS) {
-            const TV v = ((const TV*)row)[i];
+    if (vec && i + 16 <= K) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) top = max(top, __float_as_uint(Elem<DT>::get(v[e])) & 0x7fffffffu);
+        for (int p = 0; p < 16 / V; ++p) {
+            const TV v = *(const TV*)(row + i + p * V);
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[p * V + e] = Elem<DT>::get(v[e]);
         }
-        for (int i = nv * V + t; i < K; i += THREADS) top = max(top, __float_as_uint(Elem<DT>::get(row[i])) & 0x7fffffffu);
     } else {
-        for (int i = t; i < K; i += THREADS) top = max(top, __float_as_uint(Elem<DT>::get(row[i])) & 0x7fffffffu);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) f[e] = i + e < K ? Elem<DT>::get(row[i + e]) : 0.0f;
     }
+}
+
+template <int THREADS>
+__device__ __forceinline__ unsigned row_top(unsigned top, unsigned* part) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
-    if ((t & 63) == 0) part[t >> 6] = top;
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < THREADS / 64; ++w) top = max(top, part[w]);
+    return top;
+}
+
+// scale of the row and 127 / amax (0 where there is nothing to scale).  A row that holds a NaN or an infinity gets the
+// scale NaN and zeros, so every y of it is NaN.
+__device__ __forceinline__ double row_scale(unsigned top, float* scale) {
     const float amax = __uint_as_float(top);
     const bool finite = top < 0x7f800000u;
-    if (t == 0) scale[blockIdx.x] = finite ? amax / 127.0f : __uint_as_float(0x7fc00000u);
-    const double inv = finite && amax > 0.0f ? 127.0 / (double)amax : 0.0;
-    // 16 results at a time (q and ldq are multiples of 16 bytes)
-    for (int i = t * 16; i < Kz; i += THREADS * 16) {
-        float v[16];
-        if (vec && i + 16 <= K) {
+    if (threadIdx.x == 0) *scale = finite ? amax / 127.0f : __uint_as_float(0x7fc00000u);
+    return finite && top ? 127.0 / (double)amax : 0.0;
+}
+
+union Quantized {
+    v4i w;
+    int8_t b[16];
+};
+
+// One workgroup per row, a thread 16 numbers at a time, held in registers between the maximum and the division
+// (K <= THREADS * 16 * CHUNKS): every byte is read once and a row costs one trip to memory.  Zeros are written from K to
+// Kz, a multiple of 16: the padding the product's blocks of 128 bytes read.  8,192 rows of 4,096 bf16: @Q@.
+template <int DT, int THREADS, int CHUNKS>
+__global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const typename Elem<DT>::T* __restrict__ x, long long ldx,
+                                                                int8_t* __restrict__ q, long long ldq,
+                                                                float* __restrict__ scale, int K, int Kz, int vec) {
+    __shared__ unsigned part[THREADS / 64];
+    const typename Elem<DT>::T* row = x + (long long)blockIdx.x * ldx;
+    int8_t* out = q + (long long)blockIdx.x * ldq;
+    float v[CHUNKS][16];
 #pragma unroll
-            for (int c = 0; c < 16 / V; ++c) {
-                const TV u = *(const TV*)(row + i + c * V);
+    for (int c = 0; c < CHUNKS; ++c) load16<DT>(row, (c * THREADS + (int)threadIdx.x) * 16, K, vec, v[c]);
+    unsigned top = 0;
 #pragma unroll
-                for (int e = 0; e < V; ++e) v[c * V + e] = Elem<DT>::get(u[e]);
-            }
-        } else {
+    for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = i + e < K ? Elem<DT>::get(row[i + e]) : 0.0f;
+        for (int e = 0; e < 16; ++e) top = max(top, magnitude(v[c][e]));
+    const double inv = row_scale(row_top<THREADS>(top, part), scale + blockIdx.x);
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+        const int at = (c * THREADS + (int)threadIdx.x) * 16;
+        if (at >= Kz) break;
+        Quantized o;
+        o.w = v4i{0, 0, 0, 0};
+        if (inv > 0.0) quantize_some(v[c], inv, o.b);
+        *(v4i*)(out + at) = o.w;
+    }
+}
+
+// Few long rows: a CU alone takes 4 us to bring in 100 KB, so PARTS workgroups share a row in two launches, the largest
+// magnitudes of the parts first (tops: rows x PARTS).  64 rows of 50,176: @P@ instead of 11 us.
+constexpr int QUANT_PARTS = 16;
+
+template <int DT>
+__global__ __launch_bounds__(256) void quantize_top_kernel(const typename Elem<DT>::T* __restrict__ x, long long ldx,
+                                                           unsigned* __restrict__ tops, int K, int span) {
+    __shared__ unsigned part[4];
+    const typename Elem<DT>::T* row = x + (long long)blockIdx.y * ldx;
+    const int from = (int)blockIdx.x * span, to = from + span < K ? from + span : K;
+    unsigned top = 0;
+    for (int i = from + (int)threadIdx.x * 16; i < to; i += 4096) {
+        float f[16];
+        load16<DT>(row, i, K, true, f);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = max(top, magnitude(f[e]));
+    }
+    top = row_top<256>(top, part);
+    if (threadIdx.x == 0) tops[blockIdx.y * QUANT_PARTS + blockIdx.x] = top;
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void quantize_part_kernel(const typename Elem<DT>::T* __restrict__ x, long long ldx,
+                                                            int8_t* __restrict__ q, long long ldq, float* __restrict__ scale,
+                                                            const unsigned* __restrict__ tops, int K, int Kz, int span) {
+    const typename Elem<DT>::T* row = x + (long long)blockIdx.y * ldx;
+    int8_t* out = q + (long long)blockIdx.y * ldq;
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < QUANT_PARTS; ++i) top = max(top, tops[blockIdx.y * QUANT_PARTS + i]);
+    const float amax = __uint_as_float(top);
+    const bool finite = top < 0x7f800000u;
+    if (blockIdx.x == 0 && threadIdx.x == 0) scale[blockIdx.y] = finite ? amax / 127.0f : __uint_as_float(0x7fc00000u);
+    const double inv = finite && top ? 127.0 / (double)amax : 0.0;
+    const int from = (int)blockIdx.x * span, to = from + span < Kz ? from + span : Kz;
+    for (int i = from + (int)threadIdx.x * 16; i < to; i += 4096) {
+        Quantized o;
+        o.w = v4i{0, 0, 0, 0};
+        if (inv > 0.0) {
+            float f[16];
+            load16<DT>(row, i, K, true, f);
+            quantize_some(f, inv, o.b);
         }
-        union {
-            v4i w;
-            int8_t b[16];
-        } o;
+        *(v4i*)(out + i) = o.w;
+    }
+}
+
+// rows of any length: read twice, the second time out of L2
+template <int DT>
+__global__ __launch_bounds__(1024) void quantize_long_rows_kernel(const typename Elem<DT>::T* __restrict__ x, long long ldx,
+                                                                 int8_t* __restrict__ q, long long ldq,
+                                                                 float* __restrict__ scale, int K, int Kz) {
+    __shared__ unsigned part[16];
+    const typename Elem<DT>::T* row = x + (long long)blockIdx.x * ldx;
+    int8_t* out = q + (long long)blockIdx.x * ldq;
+    unsigned top = 0;
+    for (int i = threadIdx.x; i < K; i += 1024) top = max(top, magnitude(Elem<DT>::get(row[i])));
+    const double inv = row_scale(row_top<1024>(top, part), scale + blockIdx.x);
+    for (int i = threadIdx.x * 4; i < Kz; i += 4096) {
+        unsigned o = 0;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o.b[e] = (int8_t)(finite ? quantize_one(v[e], inv) : 0);
-        if (i + 16 <= Kz) *(v4i*)(out + i) = o.w;
-        else
-            for (int e = 0; e < Kz - i; ++e) out[i + e] = o.b[e];
+        for (int e = 0; e < 4; ++e)
+            if (i + e < K && inv > 0.0) o |= (unsigned)(uint8_t)(int8_t)quantize_one(Elem<DT>::get(row[i + e]), inv) << (8 * e);
+        *(unsigned*)(out + i) = o;
     }
 }
 
@@ -156,8 +260,34 @@ struct LinearI8Args {
     int blocks;             // of 128 bytes along K
     int slices, per_slice;  // the contraction in slices of per_slice blocks
     int tiles_m, tiles_n;
-    int whole;              // four neighbours of a row of y may be stored at once
+    int store;              // how a row of y is stored
 };
+
+enum { STORE_ONE = 0, STORE_PAIR = 1, STORE_16 = 2 };   // rows lie on their numbers' size, on twice that, on 16 bytes
+
+// WIDTH neighbouring numbers of a row of y (rows x cols), as one store where they are all inside
+template <int DT, int WIDTH>
+__device__ __forceinline__ void put_row(typename Elem<DT>::T* y, long long row, long long col, long long rows, long long cols,
+                                        long long ld, const float (&v)[WIDTH]) {
+    typedef typename Elem<DT>::T T;
+    if (row >= rows) return;
+    T* p = y + row * ld + col;
+    if (col + WIDTH <= cols) {
+        if constexpr (WIDTH == 1) {
+            *p = Elem<DT>::put(v[0]);
+        } else {
+            typedef T TV __attribute__((ext_vector_type(WIDTH)));
+            TV o;
+#pragma unroll
+            for (int e = 0; e < WIDTH; ++e) o[e] = Elem<DT>::put(v[e]);
+            *(TV*)p = o;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < WIDTH; ++e)
+            if (col + e < cols) p[e] = Elem<DT>::put(v[e]);
+    }
+}
 
 template <int DT>
 __device__ __forceinline__ void linear_store(const LinearI8Args& a, long long m, long long n, const v4i& d) {
@@ -171,7 +301,7 @@ __device__ __forceinline__ void linear_store(const LinearI8Args& a, long long m,
             v[r] = (float)d[r] * s * a.sw[n + r];
             if (a.bias) v[r] += a.bias[n + r];
         }
-    put4<DT>((typename Elem<DT>::T*)a.y + m * a.ldy + n, v, left, a.whole);
+    put4<DT>((typename Elem<DT>::T*)a.y + m * a.ldy + n, v, left, a.store == STORE_16);
 }
 
 template <int DT, int BM, int BN, int WM, int WN, int STAGES>
@@ -194,31 +324,181 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_i8_tile_kernel(LinearI
     const int k1 = k0 + a.per_slice < a.blocks ? k0 + a.per_slice : a.blocks;
     P::run(A, B, k0, k1, ring, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long m0 = tm * BM + (wave / WN) * (BM / WM) + piece_across(lane);
-    const long long n0 = tn * BN + (wave % WN) * (BN / WN) + piece_along(lane);
+    const long long mw = tm * BM + (wave / WN) * (BM / WM), nw = tn * BN + (wave % WN) * (BN / WN);
+    const long long m0 = mw + piece_across(lane), n0 = nw + piece_along(lane);
+    if (a.slices > 1) {
 #pragma unroll
-    for (int i = 0; i < P::TM; ++i)
+        for (int i = 0; i < P::TM; ++i)
 #pragma unroll
-        for (int j = 0; j < P::TN; ++j) {
-            const long long m = m0 + i * 16, n = n0 + j * 16;
-            if (a.slices == 1) {
-                linear_store<DT>(a, m, n, acc[i][j]);
-            } else if (m < a.M) {
+            for (int j = 0; j < P::TN; ++j) {
+                const long long m = m0 + i * 16, n = n0 + j * 16;
+                if (m >= a.M) continue;
                 int* p = a.partial + ((long long)slice * a.M + m) * a.N + n;
+                if (a.N % 4 == 0) {
+                    if (n < a.N) *(v4i*)p = acc[i][j];
+                } else {
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (n + r < a.N) p[r] = acc[i][j][r];
+                    for (int r = 0; r < 4; ++r)
+                        if (n + r < a.N) p[r] = acc[i][j][r];
+                }
             }
+        return;
+    }
+    typedef typename Elem<DT>::T T;
+    float w[P::TN][4], b[P::TN][4];
+#pragma unroll
+    for (int j = 0; j < P::TN; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const long long n = n0 + j * 16 + r < a.N ? n0 + j * 16 + r : a.N - 1;
+            w[j][r] = a.sw[n];
+            b[j][r] = a.bias ? a.bias[n] : 0.0f;
         }
+    __syncthreads();
+    static_assert((P::WAVES + 1) / 2 * TURN_BYTES<P::TN> <= P::HALF, "fits two stages");
+    LdsPtr turn = (wave & 1 ? ring[1] : ring[0]) + (wave >> 1) * TURN_BYTES<P::TN>;
+#pragma unroll
+    for (int i = 0; i < P::TM; ++i) {
+        const long long m = m0 + i * 16;
+        const float s = a.sx[m < a.M ? m : a.M - 1];
+        float v[P::TN][4];
+#pragma unroll
+        for (int j = 0; j < P::TN; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                v[j][r] = (float)acc[i][j][r] * s * w[j][r];
+                if (a.bias) v[j][r] += b[j][r];
+            }
+        turn_in<P::TN>(turn, v);
+        auto emit = [&](int row, int col, const auto& x) { put_row<DT>((T*)a.y, mw + i * 16 + row, nw + col, a.M, a.N, a.ldy, x); };
+        if (a.store == STORE_16) turn_out<P::TN, 16 / (int)sizeof(T)>(turn, emit);
+        else if (sizeof(T) == 2 && a.store == STORE_PAIR) turn_out<P::TN, 2>(turn, emit);
+        else turn_out<P::TN, 1>(turn, emit);
+    }
 }
 
 // the slices' sums (integers: any order gives the same), scales, bias
+// Up to 16 rows: the weight is read once, straight into registers, and that is what bounds it.  A workgroup of 16
+// wavefronts takes 16 channels; a wavefront takes every 16th block of 128 bytes of their rows, four blocks (8 KB) on
+// their way while four are worked on; the 16 sums meet in LDS.  QUANTIZE: the rows of x are quantised by every
+// workgroup for itself, into LDS, while its first weights are on their way: that costs less than a launch up to
+// 65,536 numbers, which is what a workgroup holds.  @ROWS@
+template <int DTX, int DT, bool QUANTIZE>
+__global__ __launch_bounds__(1024) void linear_i8_rows_kernel(LinearI8Args a, const typename Elem<DTX>::T* __restrict__ x,
+                                                              long long ldx, int K, int vec) {
+    typedef typename Elem<DTX>::T T;
+    constexpr int AHEAD = 4, WAVES = 16;
+    extern __shared__ __align__(16) char rows_lds[];        // QUANTIZE: M rows of a.blocks * 128 bytes
+    __shared__ __align__(16) v4i sums[WAVES][64];
+    __shared__ unsigned part[WAVES];
+    __shared__ float row_s[16];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int lr = lane & 15, lq = (lane >> 4) * 16;
+    const long long n0 = (long long)blockIdx.x * 16;
+    const int M = (int)a.M;
+    const char* w = (const char*)a.w + (n0 + lr < a.N ? n0 + lr : a.N - 1) * a.ldw;
+    const int m = lr < M ? lr : M - 1;
+    const int row_bytes = a.blocks * 128;
+    const char* q = (const char*)a.q + m * a.ldq;
+    const int last = a.blocks - 1;
+    v4i wr[2][AHEAD][2];
+    auto fetch = [&](v4i (&r)[AHEAD][2], int kb) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+            if (kb + u * WAVES <= last) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int off = (kb + u * WAVES) * 128 + h * 64 + lq;
+                    r[u][h] = *(const v4i*)(w + (off < a.last_w ? off : a.last_w));
+                }
+            }
+    };
+    fetch(wr[0], wave);
+    if (QUANTIZE) {
+        // 1024 / rows threads (rounded down to a power of two) to a row, 16 numbers at a time
+        int per = 1024;
+        while (per * M > 1024) per >>= 1;
+        const int row = t / per, at0 = (t & (per - 1)) * 16;
+        const bool mine = row < M;
+        const T* xr = x + (mine ? row : 0) * ldx;
+        unsigned top = 0;
+        const int end = mine ? K : 0, pad = mine ? row_bytes : 0;
+#pragma unroll 4
+        for (int i = at0; i < end; i += per * 16) {
+            float f[16];
+            load16<DTX>(xr, i, K, vec, f);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = max(top, magnitude(f[e]));
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
+        if (lane == 0) part[wave] = top;
+        __syncthreads();
+        const int span = per / 64, first = (wave / span) * span;      // per is 64 at least: M <= 16
+        for (int i = 0; i < span; ++i) top = max(top, part[first + i]);
+        const float amax = __uint_as_float(top);
+        const bool finite = top < 0x7f800000u;
+        const double inv = finite && top ? 127.0 / (double)amax : 0.0;
+        if (mine && at0 == 0) row_s[row] = finite ? amax / 127.0f : __uint_as_float(0x7fc00000u);
+#pragma unroll 4
+        for (int i = at0; i < pad; i += per * 16) {
+            Quantized o;
+            o.w = v4i{0, 0, 0, 0};
+            if (inv > 0.0) {
+                float f[16];
+                load16<DTX>(xr, i, K, vec, f);
+                quantize_some(f, inv, o.b);
+            }
+            *(v4i*)(rows_lds + row * row_bytes + i) = o.w;
+        }
+        __syncthreads();
+    }
+    v4i acc = {0, 0, 0, 0};
+    auto work = [&](const v4i (&r)[AHEAD][2], int kb) {
+        v4i xr[AHEAD][2];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int b = kb + u * WAVES < last ? kb + u * WAVES : last;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int off = b * 128 + h * 64 + lq;
+                xr[u][h] = *(const v4i*)(QUANTIZE ? rows_lds + m * row_bytes + off : q + off);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+            if (kb + u * WAVES <= last) {
+                MathI8::mma<0>(acc, r[u], xr[u]);
+                MathI8::mma<1>(acc, r[u], xr[u]);
+            }
+    };
+    for (int kb = wave; kb <= last; kb += 2 * AHEAD * WAVES) {
+        fetch(wr[1], kb + AHEAD * WAVES);
+        work(wr[0], kb);
+        fetch(wr[0], kb + 2 * AHEAD * WAVES);
+        work(wr[1], kb + AHEAD * WAVES);
+    }
+    sums[wave][lane] = acc;
+    __syncthreads();
+    if (t < 64) {       // the channels lie along a lane's registers
+        v4i d = sums[0][lane];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) d += sums[i][lane];
+        if (lr < M) {
+            LinearI8Args b = a;
+            if (QUANTIZE) b.sx = row_s;
+            linear_store<DT>(b, lr, n0 + piece_along(lane), d);
+        }
+    }
+}
+
 template <int DT>
 __global__ __launch_bounds__(256) void linear_i8_join_kernel(LinearI8Args a) {
     const long long quads = (a.N + 3) / 4, total = a.M * quads, plane = a.M * a.N;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
         const long long m = i / quads, n = (i - m * quads) * 4;
         v4i d = {0, 0, 0, 0};
+#pragma unroll 8
         for (int s = 0; s < a.slices; ++s) {
             const int* p = a.partial + s * plane + m * a.N + n;
 #pragma unroll

@@ -185,6 +185,50 @@ struct TileProduct {
 __device__ __forceinline__ int piece_along(int lane) { return (lane >> 4) * 4; }
 __device__ __forceinline__ int piece_across(int lane) { return lane & 15; }
 
+// Sixteen rows of a wavefront's result, PIECES * 16 columns, turned through LDS so that neighbouring lanes hold
+// neighbouring columns: a lane by itself holds four numbers of a row, and stores of 8 bytes in every row cost a third of
+// a large product's time.  v[p] are the lane's four numbers of piece p; emit(row, column, numbers) is called with WIDTH
+// neighbouring numbers of a row.  `turn` is LDS of this wavefront alone (TURN_BYTES<PIECES>).
+template <int PIECES> constexpr int TURN_LINE = PIECES * 64 + 16;
+template <int PIECES> constexpr int TURN_BYTES = 16 * TURN_LINE<PIECES>;
+
+template <int PIECES>
+__device__ __forceinline__ void turn_in(LdsPtr turn, const float (&v)[PIECES][4]) {
+    const int lane = threadIdx.x & 63;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p)
+        *(__attribute__((address_space(3))) v4f*)(turn + piece_across(lane) * TURN_LINE<PIECES> + (p * 16 + piece_along(lane)) * 4) =
+            v4f{v[p][0], v[p][1], v[p][2], v[p][3]};
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <int PIECES, int WIDTH, class Emit>
+__device__ __forceinline__ void turn_out(LdsPtr turn, Emit&& emit) {
+    constexpr int PER_ROW = PIECES * 16 / WIDTH, ROWS = 64 / PER_ROW;
+    const int lane = threadIdx.x & 63, col = lane % PER_ROW * WIDTH;
+#pragma unroll
+    for (int r0 = 0; r0 < 16; r0 += ROWS) {
+        const int row = r0 + lane / PER_ROW;
+        float v[WIDTH];
+        if constexpr (WIDTH >= 4) {
+#pragma unroll
+            for (int e = 0; e < WIDTH; e += 4) {
+                const v4f t = *(const __attribute__((address_space(3))) v4f*)(turn + (ROWS <= 16 ? row : row & 15) * TURN_LINE<PIECES> + (col + e) * 4);
+                v[e] = t[0];
+                v[e + 1] = t[1];
+                v[e + 2] = t[2];
+                v[e + 3] = t[3];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < WIDTH; ++e)
+                v[e] = *(const __attribute__((address_space(3))) float*)(turn + (ROWS <= 16 ? row : row & 15) * TURN_LINE<PIECES> + (col + e) * 4);
+        }
+        if (ROWS <= 16 || row < 16) emit(row, col, v);
+    }
+}
+
 // workgroup -> tile so that the workgroups of one XCD (every eighth of the launch order) take neighbouring
 // tiles and share their operands in that XCD's L2
 __device__ __forceinline__ long long xcd_order(long long b, long long n) {

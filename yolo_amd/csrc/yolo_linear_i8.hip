@@ -20,63 +20,82 @@ inline size_t dtype_bytes(int dt) { return dt == YH_F32 ? 4 : dt == YH_I8 ? 1 : 
 
 constexpr int64_t kMaxRows = ((int64_t)1 << 22) - 1;      // a grid holds fewer than 2^32 threads, a row takes up to 1,024
 
+// tops: rows * QUANT_PARTS words for the shared form, or null (yh_quantize_rows has no workspace)
 template <int DT>
-void quantize_launch(const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int K, int Kz,
-                     hipStream_t st) {
+void quantize_launch(const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, unsigned* tops, int64_t rows, int K,
+                     int Kz, hipStream_t st) {
     typedef typename Elem<DT>::T T;
-    const int vec = aligned(x, 16) && (ldx * sizeof(T)) % 16 == 0;
-    if (K > 8192)
-        hipLaunchKernelGGL((quantize_rows_kernel<DT, 1024>), dim3((unsigned)rows), dim3(1024), 0, st, (const T*)x, ldx, q,
-                           ldq, scale, K, Kz, vec);
+    const dim3 grid((unsigned)rows);
+    const T* p = (const T*)x;
+    const int vec = aligned(x, 16) && (rows == 1 || (ldx * sizeof(T)) % 16 == 0);
+    if (K > 65536)
+        hipLaunchKernelGGL((quantize_long_rows_kernel<DT>), grid, dim3(1024), 0, st, p, ldx, q, ldq, scale, K, Kz);
+    else if (tops && vec && rows < 256 && K > 8192) {
+        const int span = ((Kz + QUANT_PARTS - 1) / QUANT_PARTS + 15) & ~15;
+        const dim3 parts(QUANT_PARTS, (unsigned)rows);
+        hipLaunchKernelGGL((quantize_top_kernel<DT>), parts, dim3(256), 0, st, p, ldx, tops, K, span);
+        hipLaunchKernelGGL((quantize_part_kernel<DT>), parts, dim3(256), 0, st, p, ldx, q, ldq, scale, (const unsigned*)tops, K,
+                           Kz, span);
+    } else if (K <= 1024)
+        hipLaunchKernelGGL((quantize_rows_kernel<DT, 64, 1>), grid, dim3(64), 0, st, p, ldx, q, ldq, scale, K, Kz, vec);
+    else if (K <= 4096)
+        hipLaunchKernelGGL((quantize_rows_kernel<DT, 256, 1>), grid, dim3(256), 0, st, p, ldx, q, ldq, scale, K, Kz, vec);
+    else if (K <= 16384)
+        hipLaunchKernelGGL((quantize_rows_kernel<DT, 1024, 1>), grid, dim3(1024), 0, st, p, ldx, q, ldq, scale, K, Kz, vec);
     else
-        hipLaunchKernelGGL((quantize_rows_kernel<DT, 256>), dim3((unsigned)rows), dim3(256), 0, st, (const T*)x, ldx, q,
-                           ldq, scale, K, Kz, vec);
+        hipLaunchKernelGGL((quantize_rows_kernel<DT, 1024, 4>), grid, dim3(1024), 0, st, p, ldx, q, ldq, scale, K, Kz, vec);
 }
 
-int quantize(const void* x, int dt, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int K, int Kz,
-             hipStream_t st) {
-    if (dt == YH_F32) quantize_launch<DT_F32>(x, ldx, q, ldq, scale, rows, K, Kz, st);
-    else if (dt == YH_F16) quantize_launch<DT_F16>(x, ldx, q, ldq, scale, rows, K, Kz, st);
-    else quantize_launch<DT_BF16>(x, ldx, q, ldq, scale, rows, K, Kz, st);
+int quantize(const void* x, int dt, int64_t ldx, int8_t* q, int64_t ldq, float* scale, unsigned* tops, int64_t rows, int K,
+             int Kz, hipStream_t st) {
+    if (dt == YH_F32) quantize_launch<DT_F32>(x, ldx, q, ldq, scale, tops, rows, K, Kz, st);
+    else if (dt == YH_F16) quantize_launch<DT_F16>(x, ldx, q, ldq, scale, tops, rows, K, Kz, st);
+    else quantize_launch<DT_BF16>(x, ldx, q, ldq, scale, tops, rows, K, Kz, st);
     return launch_status();
 }
 
-// How the product is cut: tiles of one of three sizes, and slices of the contraction.
+// How the product is cut: tiles of one of four sizes, and slices of the contraction.
 //
-//   tile      wavefronts  stages  LDS     block, one workgroup a CU / as many as fit (measured, us)
-//   128x256   8           3       144 KB  1.27
-//   128x128   8           4       128 KB  0.63
-//   64x64     4           3        48 KB  0.40 / 0.61 (three)
+//   tile      wavefronts  stages  LDS     workgroups a CU   us for a block of 128 bytes: one workgroup on a CU, each more
+//   256x128   8           3       144 KB  1                 1.08
+//   128x128   8           4       128 KB  1                 0.65
+//   64x64     4           4        64 KB  2                 0.30, 0.14
+//   32x32     4           4        32 KB  5                 0.14, 0.08
 //
 // A larger tile reads less per product (a CU takes in about 64 bytes a cycle), a smaller one fills the card when
 // there are few rows or channels.  The choice is the least time of: rounds of workgroups over the 256 CUs, times the
-// blocks of a slice (+ 3 us to start and end), plus, when the sums are joined, a launch and the traffic of the partial
-// sums.  One image never comes here (linear_i8_rows_kernel).
+// blocks of a slice (+ 3 us to start and end), or the operands at 5 TB/s; plus, when the sums are joined, a launch and
+// the traffic of the partial sums.  Measured (us, 32x32 / 64x64 / 128x128 / 256x128, each with its best slices):
+// 64 x 4096 -> 1470 7.4 / 11.1 / 13.4 / -, 256 x 4096 -> 1470 8.4 / 10.3 / 17.9 / 26.3, 1024 x 4096 -> 4096 49.7 / 29.6 /
+// 23.5 / 31.7, 512 x 50,176 -> 4096 353 / 205 / 132 / 119, 8192 x 4096 -> 4096 369 / 225 / 182 / 148.
 struct Tile {
     int bm, bn, per_cu;
-    double alone, shared;
+    double block, more;
 };
-constexpr Tile kTiles[3] = {{128, 256, 1, 1.27, 1.27}, {128, 128, 1, 0.63, 0.63}, {64, 64, 3, 0.40, 0.61}};
+constexpr int kTileKinds = 4;
+constexpr Tile kTiles[kTileKinds] = {{256, 128, 1, 1.08, 0.0}, {128, 128, 1, 0.65, 0.0}, {64, 64, 2, 0.30, 0.14}, {32, 32, 5, 0.14, 0.08}};
 
 struct Plan {
     int tile, tiles_m, tiles_n, slices, per_slice, blocks;
-    size_t q_off, s_off, p_off, total;
+    size_t q_off, s_off, t_off, p_off, total;
 };
 
 Plan plan_for(int64_t M, int64_t N, int64_t K) {
     Plan p = {};
     p.blocks = (int)((K + 127) / 128);
     double best = 0.0;
-    for (int t = 0; t < 3; ++t) {
+    const double operands = ((double)N + (double)M) * (double)K / 5e6;
+    for (int t = 0; t < kTileKinds; ++t) {
         const Tile& c = kTiles[t];
         const int64_t tm = (M + c.bm - 1) / c.bm, tn = (N + c.bn - 1) / c.bn, tiles = tm * tn;
         for (int s = 1; s <= 16 && s <= p.blocks; s *= 2) {
             if (s > 1 && tiles * s > 2048) break;
             const int64_t wgs = tiles * s, at_once = 256 * (int64_t)c.per_cu;
             const int per = (p.blocks + s - 1) / s;
-            const double block = wgs <= 256 ? c.alone : c.shared;
-            double us = (double)((wgs + at_once - 1) / at_once) * (per * block + 3.0);
-            if (s > 1) us += 3.0 + (double)(s + 1) * (double)M * (double)N * 4.0 / 4e6;
+            const int64_t together = wgs >= at_once ? c.per_cu : (wgs + 255) / 256;
+            double us = (double)((wgs + at_once - 1) / at_once) * (per * (c.block + c.more * (double)(together - 1)) + 3.0);
+            if (us < operands + 3.0) us = operands + 3.0;
+            if (s > 1) us += 4.0 + (double)(s + 1) * (double)M * (double)N * 4.0 / 3e6;
             if (best == 0.0 || us < best) {
                 best = us;
                 p.tile = t;
@@ -89,9 +108,31 @@ Plan plan_for(int64_t M, int64_t N, int64_t K) {
     }
     p.q_off = 0;
     p.s_off = up256((size_t)M * p.blocks * 128);
-    p.p_off = p.s_off + up256((size_t)M * 4);
+    p.t_off = p.s_off + up256((size_t)M * 4);
+    p.p_off = p.t_off + (M < 256 ? up256((size_t)M * QUANT_PARTS * 4) : 0);
     p.total = p.p_off + (p.slices > 1 ? up256((size_t)p.slices * M * N * 4) : 0);
     return p;
+}
+
+constexpr int kRows = 16;      // rows linear_i8_rows_kernel takes
+// It quantises them itself when that is less than a launch by itself (us, with / without: 1 x 4096 5.7 / 7.1, 4 x 4096
+// 8.0 / 7.8, 16 x 4096 14.2 / 8.9, 1 x 50,176 46.1 / 50.5); they have to fit its LDS.
+inline bool quantizes_itself(int64_t M, int64_t blocks) { return blocks <= 512 && (M == 1 || M * blocks <= 96); }
+
+template <int DTX, int DT, bool QUANTIZE>
+int few_rows(const LinearI8Args& a, const void* x, int64_t ldx, int K, hipStream_t st) {
+    hipLaunchKernelGGL((linear_i8_rows_kernel<DTX, DT, QUANTIZE>), dim3((unsigned)((a.N + 15) / 16)), dim3(1024),
+                       QUANTIZE ? (size_t)a.M * a.blocks * 128 : 0, st, a, (const typename Elem<DTX>::T*)x, ldx, K,
+                       aligned(x, 16) && (a.M == 1 || (ldx * sizeof(typename Elem<DTX>::T)) % 16 == 0));
+    return launch_status();
+}
+
+template <int DT>
+int few_rows_of(const LinearI8Args& a, const void* x, int x_dtype, int64_t ldx, int K, hipStream_t st) {
+    if (x_dtype == YH_F32) return few_rows<DT_F32, DT, true>(a, x, ldx, K, st);
+    if (x_dtype == YH_F16) return few_rows<DT_F16, DT, true>(a, x, ldx, K, st);
+    if (x_dtype == YH_BF16) return few_rows<DT_BF16, DT, true>(a, x, ldx, K, st);
+    return few_rows<DT_F32, DT, false>(a, nullptr, 0, K, st);      // a.q holds the rows
 }
 
 template <int DT, int BM, int BN, int WM, int WN, int STAGES>
@@ -102,9 +143,10 @@ void tiles(const LinearI8Args& a, hipStream_t st) {
 
 template <int DT>
 int product(int tile, const LinearI8Args& a, hipStream_t st) {
-    if (tile == 0) tiles<DT, 128, 256, 2, 4, 3>(a, st);
+    if (tile == 0) tiles<DT, 256, 128, 4, 2, 3>(a, st);
     else if (tile == 1) tiles<DT, 128, 128, 2, 4, 4>(a, st);
-    else tiles<DT, 64, 64, 2, 2, 3>(a, st);
+    else if (tile == 2) tiles<DT, 64, 64, 2, 2, 4>(a, st);
+    else tiles<DT, 32, 32, 2, 2, 4>(a, st);
     if (const int rc = launch_status()) return rc;
     if (a.slices > 1) {
         int64_t b = (a.M * ((a.N + 3) / 4) + 255) / 256;
@@ -116,7 +158,7 @@ int product(int tile, const LinearI8Args& a, hipStream_t st) {
 
 int check_sizes(int64_t M, int64_t N, int64_t K) {
     if (M < 0 || N < 0 || K < 1 || K > YH_MAX_I8_K || M > kMaxRows || N > kMaxRows) return YH_ERR_SHAPE;
-    if (((M + 63) / 64) * ((N + 63) / 64) >= ((int64_t)1 << 22)) return YH_ERR_SHAPE;      // 512 threads a tile
+    if (((M + 31) / 32) * ((N + 31) / 32) >= ((int64_t)1 << 24)) return YH_ERR_SHAPE;      // 256 threads a tile
     return YH_OK;
 }
 
@@ -133,7 +175,7 @@ int yh_quantize_rows(const void* x, int x_dtype, int64_t ldx, int8_t* q, int64_t
     if (!aligned(x, dtype_bytes(x_dtype)) || !aligned(scale, 4) || !aligned(q, 16) || ldq % 16 != 0) return YH_ERR_ALIGN;
     int64_t Kz = (K + 127) / 128 * 128;
     if (Kz > ldq) Kz = ldq;
-    return quantize(x, x_dtype, ldx, q, ldq, scale, rows, (int)K, (int)Kz, (hipStream_t)stream);
+    return quantize(x, x_dtype, ldx, q, ldq, scale, nullptr, rows, (int)K, (int)Kz, (hipStream_t)stream);
 }
 
 size_t yh_linear_i8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
@@ -161,21 +203,6 @@ int yh_linear_i8(const void* x, int x_dtype, int64_t ldx, const float* x_scale, 
     a.q = (const int8_t*)(ws + p.q_off);
     a.ldq = (long long)p.blocks * 128;
     a.sx = (const float*)(ws + p.s_off);
-    if (x_dtype != YH_I8) {
-        const int rc = quantize(x, x_dtype, ldx, (int8_t*)(ws + p.q_off), a.ldq, (float*)(ws + p.s_off), M, (int)K,
-                                (int)a.ldq, st);
-        if (rc) return rc;
-    } else {
-        a.sx = x_scale;
-        if (K % 128 == 0 && ldx % 16 == 0 && aligned(x, 16)) {
-            a.q = (const int8_t*)x;
-            a.ldq = ldx;
-        } else {
-            hipLaunchKernelGGL(repack_rows_kernel, dim3((unsigned)M), dim3(256), 0, st, (const int8_t*)x, ldx,
-                               (int8_t*)(ws + p.q_off), a.ldq, (int)K, (int)a.ldq);
-            if (const int rc = launch_status()) return rc;
-        }
-    }
     a.w = w;
     a.ldw = ldw;
     a.sw = w_scale;
@@ -191,7 +218,34 @@ int yh_linear_i8(const void* x, int x_dtype, int64_t ldx, const float* x_scale, 
     a.per_slice = p.per_slice;
     a.tiles_m = p.tiles_m;
     a.tiles_n = p.tiles_n;
-    a.whole = (ldy * dtype_bytes(y_dtype)) % (4 * dtype_bytes(y_dtype)) == 0 && aligned(y, 4 * dtype_bytes(y_dtype));
+    const size_t e = dtype_bytes(y_dtype);
+    a.store = (ldy * e) % 16 == 0 && aligned(y, 16) ? STORE_16 : ldy % 2 == 0 && aligned(y, 2 * e) ? STORE_PAIR : STORE_ONE;
+    if (x_dtype != YH_I8 && M <= kRows && quantizes_itself(M, p.blocks)) {
+        if (y_dtype == YH_F32) return few_rows_of<DT_F32>(a, x, x_dtype, ldx, (int)K, st);
+        if (y_dtype == YH_F16) return few_rows_of<DT_F16>(a, x, x_dtype, ldx, (int)K, st);
+        return few_rows_of<DT_BF16>(a, x, x_dtype, ldx, (int)K, st);
+    }
+    if (x_dtype != YH_I8) {
+        const int rc = quantize(x, x_dtype, ldx, (int8_t*)(ws + p.q_off), a.ldq, (float*)(ws + p.s_off),
+                                (unsigned*)(ws + p.t_off), M, (int)K,
+                                (int)a.ldq, st);
+        if (rc) return rc;
+    } else {
+        a.sx = x_scale;
+        if (K % 128 == 0 && ldx % 16 == 0 && aligned(x, 16)) {
+            a.q = (const int8_t*)x;
+            a.ldq = ldx;
+        } else {
+            hipLaunchKernelGGL(repack_rows_kernel, dim3((unsigned)M), dim3(256), 0, st, (const int8_t*)x, ldx,
+                               (int8_t*)(ws + p.q_off), a.ldq, (int)K, (int)a.ldq);
+            if (const int rc = launch_status()) return rc;
+        }
+    }
+    if (M <= kRows) {
+        if (y_dtype == YH_F32) return few_rows_of<DT_F32>(a, nullptr, YH_I8, 0, (int)K, st);
+        if (y_dtype == YH_F16) return few_rows_of<DT_F16>(a, nullptr, YH_I8, 0, (int)K, st);
+        return few_rows_of<DT_BF16>(a, nullptr, YH_I8, 0, (int)K, st);
+    }
     if (y_dtype == YH_F32) return product<DT_F32>(p.tile, a, st);
     if (y_dtype == YH_F16) return product<DT_F16>(p.tile, a, st);
     return product<DT_BF16>(p.tile, a, st);

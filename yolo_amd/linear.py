@@ -8,6 +8,7 @@ the input (an image's features) and of the weight (an output channel).
 The sum is exact in int32; scales and bias are applied in fp32.  Forward only."""
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -17,6 +18,11 @@ from . import _lib
 from ._tensors import _need, _on_device, _ptr, _stream
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+@lru_cache(maxsize=4096)
+def _workspace_bytes(m: int, n: int, k: int) -> int:
+    return _lib.load().yh_linear_i8_workspace_bytes(m, n, k)
 
 
 def _no_grad(t: torch.Tensor, name: str) -> None:
@@ -112,10 +118,9 @@ def linear_i8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
     y = torch.empty(*shape[:-1], n, dtype=out_dtype, device=dev)
     if y.numel() == 0:
         return y
-    lib = _lib.load()
-    ws = torch.empty(lib.yh_linear_i8_workspace_bytes(m, n, k), dtype=torch.uint8, device=dev)
+    ws = torch.empty(_workspace_bytes(m, n, k), dtype=torch.uint8, device=dev)
     with _on_device(dev):
-        _lib.check(lib.yh_linear_i8(x.data_ptr(), _lib.DTYPE_CODES[x.dtype], _ld(x), _ptr(x_scale), weight.data_ptr(), ldw,
+        _lib.check(_lib.load().yh_linear_i8(x.data_ptr(), _lib.DTYPE_CODES[x.dtype], _ld(x), _ptr(x_scale), weight.data_ptr(), ldw,
                                     weight_scale.data_ptr(), _ptr(bias), y.data_ptr(), _lib.DTYPE_CODES[out_dtype], n, m, n,
                                     k, ws.data_ptr(), ws.numel(), _stream(dev)))
     return y
