@@ -289,6 +289,24 @@ __device__ __forceinline__ void put_row(typename Elem<DT>::T* y, long long row, 
     }
 }
 
+// the same from a matrix without gaps between rows; zeros past its columns
+template <int DT, int WIDTH>
+__device__ __forceinline__ void get_row(const typename Elem<DT>::T* y, long long row, long long col, long long cols, float (&v)[WIDTH]) {
+    typedef typename Elem<DT>::T T;
+    const T* p = y + row * cols + col;
+    if constexpr (WIDTH > 1) {
+        if (col + WIDTH <= cols) {
+            typedef T TV __attribute__((ext_vector_type(WIDTH)));
+            const TV o = *(const TV*)p;
+#pragma unroll
+            for (int e = 0; e < WIDTH; ++e) v[e] = Elem<DT>::get(o[e]);
+            return;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < WIDTH; ++e) v[e] = col + e < cols ? Elem<DT>::get(p[e]) : 0.0f;
+}
+
 template <int DT>
 __device__ __forceinline__ void linear_store(const LinearI8Args& a, long long m, long long n, const v4i& d) {
     if (m >= a.M || n >= a.N) return;

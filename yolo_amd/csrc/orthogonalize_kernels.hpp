@@ -76,87 +76,184 @@ __device__ __forceinline__ double block_sum(double v, double* part) {
 
 // ---------------------------------------------------------------- norm (and momentum)
 // Squares are added in 64 bits: no gradient in fp32 range overflows or vanishes.  One partial sum per workgroup, added
-// in order by whoever needs the norm: the same bits from run to run.
+// in order by whoever needs the norm: the same bits from run to run.  vec: matrices without gaps between rows, on 16 bytes
+// and of a multiple of eight numbers; a thread then takes eight at a time.  @NORM@
 template <int DT, bool LIST>
-__global__ __launch_bounds__(256) void ns_norm_kernel(NsSource src, NsShape sh, double* __restrict__ parts) {
+__global__ __launch_bounds__(256) void ns_norm_kernel(NsSource src, NsShape sh, double* __restrict__ parts, int vec) {
     __shared__ double part[4];
     const int mat = blockIdx.y;
-    const long long total = sh.rows * sh.cols;
+    const long long total = sh.rows * sh.cols, stride = (long long)gridDim.x * 256;
     typedef typename Elem<DT>::T T;
     const T* g = LIST ? (const T*)src.g[mat] : (const T*)src.base + mat * src.stride_b;
-    const bool flat = LIST || src.stride_r == sh.cols;
+    float* buf = LIST ? src.buf[mat] : nullptr;
     double sum = 0.0;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        long long at = i;
-        if (!flat) {
-            const long long r = i / sh.cols;
-            at = r * src.stride_r + (i - r * sh.cols);
-        }
-        float v = Elem<DT>::get(g[at]);
+    auto one = [&](float v, float* m) {
         if (LIST) {
-            const float m = src.momentum * src.buf[mat][i] + v;
-            src.buf[mat][i] = m;
-            v = src.nesterov ? v + src.momentum * m : m;
+            *m = src.momentum * *m + v;
+            v = src.nesterov ? v + src.momentum * *m : *m;
         }
         sum += (double)v * (double)v;
+    };
+    if (vec) {
+        constexpr int V = 16 / (int)sizeof(T);
+        typedef T TV __attribute__((ext_vector_type(V)));
+#pragma unroll 2
+        for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i * 8 < total; i += stride) {
+            TV v[8 / V];
+            v4f m[2];
+#pragma unroll
+            for (int p = 0; p < 8 / V; ++p) v[p] = *(const TV*)(g + i * 8 + p * V);
+            if (LIST) {
+                m[0] = *(const v4f*)(buf + i * 8);
+                m[1] = *(const v4f*)(buf + i * 8 + 4);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                float x = LIST ? m[e / 4][e % 4] : 0.0f;
+                one(Elem<DT>::get(v[e / V][e % V]), &x);
+                if (LIST) m[e / 4][e % 4] = x;
+            }
+            if (LIST) {
+                *(v4f*)(buf + i * 8) = m[0];
+                *(v4f*)(buf + i * 8 + 4) = m[1];
+            }
+        }
+    } else {
+        const bool flat = LIST || src.stride_r == sh.cols;
+        for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += stride) {
+            long long at = i;
+            if (!flat) {
+                const long long r = i / sh.cols;
+                at = r * src.stride_r + (i - r * sh.cols);
+            }
+            one(Elem<DT>::get(g[at]), buf + i);
+        }
     }
     sum = block_sum(sum, part);
     if (threadIdx.x == 0) parts[(long long)mat * gridDim.x + blockIdx.x] = sum;
 }
 
+// eight neighbours of a split row
+struct Split8 {
+    v4i hi, lo;
+};
+__device__ __forceinline__ Split8 split8_of(const float (&v)[8]) {
+    union {
+        v4i w;
+        _Float16 h[8];
+    } hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) split_of(v[e], hi.h[e], lo.h[e]);
+    return {hi.w, lo.w};
+}
+__device__ __forceinline__ void split8_put(char* p, const float (&v)[8]) {
+    const Split8 x = split8_of(v);
+    *(v4i*)p = x.hi;
+    *(v4i*)(p + 64) = x.lo;
+}
+// the same of v[from .. to) only
+__device__ __forceinline__ void split8_put_some(char* p, const float (&v)[8], long long from, long long to) {
+    if (from <= 0 && to >= 8) {
+        split8_put(p, v);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e >= from && e < to) {
+            _Float16 hi, lo;
+            split_of(v[e], hi, lo);
+            *(_Float16*)(p + 2 * e) = hi;
+            *(_Float16*)(p + 2 * e + 64) = lo;
+        }
+}
+// N (a power of two up to 8) neighbours, from a multiple of N on
+template <int N>
+__device__ __forceinline__ void split_get_n(const char* p, float (&v)[N]) {
+    typedef _Float16 H __attribute__((ext_vector_type(N)));
+    if constexpr (N == 1) {
+        v[0] = (float)*(const _Float16*)p + (float)*(const _Float16*)(p + 64);
+    } else {
+        const H hi = *(const H*)p, lo = *(const H*)(p + 64);
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = (float)hi[e] + (float)lo[e];
+    }
+}
+
 // ---------------------------------------------------------------- G -> X and X', split
-// 64 x 64 numbers of G per workgroup; `nat` gets G's own rows, `tra` its columns, both times scale / (|G| + eps)
+// 64 x 64 numbers of G per workgroup; `nat` gets G's own rows, `tra` its columns, both times scale / (|G| + eps).  vec: rows
+// of G (and of the momentum) on 16 bytes and of a multiple of eight numbers.  @CONVERT@
 template <int DT, bool LIST>
 __global__ __launch_bounds__(256) void ns_convert_kernel(NsSource src, NsShape sh, const double* __restrict__ parts, int nparts,
                                                          double eps, double scale, char* __restrict__ nat, long long nat_mat,
-                                                         char* __restrict__ tra, long long tra_mat) {
+                                                         char* __restrict__ tra, long long tra_mat, int vec) {
     typedef typename Elem<DT>::T T;
     __shared__ float tile[64][65];
     __shared__ double part[4];
     const int mat = blockIdx.y, t = threadIdx.x;
-    const double sq = block_sum(t < nparts ? parts[(long long)mat * nparts + t] : 0.0, part);
-    const double inv = scale / (sqrt(sq) + eps);
     const T* g = LIST ? (const T*)src.g[mat] : (const T*)src.base + mat * src.stride_b;
+    const float* buf = LIST ? src.buf[mat] : nullptr;
     const long long stride = LIST ? sh.cols : src.stride_r;
     const long long ncp = (sh.cols + 31) & ~31ll, nrp = (sh.rows + 31) & ~31ll;
     const unsigned across = (unsigned)((sh.cols + 63) / 64);
     const long long r0 = (long long)(blockIdx.x / across) * 64, c0 = (long long)(blockIdx.x % across) * 64;
-    for (int i = t; i < 4096; i += 256) {
-        const int r = i >> 6, c = i & 63;
-        float v = 0.0f;
-        if (r0 + r < sh.rows && c0 + c < sh.cols) {
-            v = Elem<DT>::get(g[(r0 + r) * stride + c0 + c]);
-            if (LIST) {
-                const float m = src.buf[mat][(r0 + r) * sh.cols + c0 + c];
-                v = src.nesterov ? v + src.momentum * m : m;
-            }
-            v = (float)((double)v * inv);
-        }
-        tile[r][c] = v;
-    }
-    __syncthreads();
     const int line = t >> 2, at = (t & 3) * 16;      // 16 numbers of a line of the tile
-    union Pack {
-        v4i w[2];
-        _Float16 h[16];
-    } hi, lo;
-    if (r0 + line < sh.rows && c0 + at < ncp) {
+    float v[16], m[16];
+    const bool row_in = r0 + line < sh.rows;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) split_of(tile[line][at + e], hi.h[e], lo.h[e]);
-        char* p = nat + mat * nat_mat + split_at(r0 + line, ncp * 4, c0 + at);
-        *(v4i*)p = hi.w[0];
-        *(v4i*)(p + 16) = hi.w[1];
-        *(v4i*)(p + 64) = lo.w[0];
-        *(v4i*)(p + 80) = lo.w[1];
+    for (int e = 0; e < 16; ++e) v[e] = m[e] = 0.0f;
+    if (vec) {
+        constexpr int V = 16 / (int)sizeof(T);
+        typedef T TV __attribute__((ext_vector_type(V)));
+#pragma unroll
+        for (int e = 0; e < 16; e += 8)
+            if (row_in && c0 + at + e < sh.cols) {
+#pragma unroll
+                for (int p = 0; p < 8; p += V) {
+                    const TV x = *(const TV*)(g + (r0 + line) * stride + c0 + at + e + p);
+#pragma unroll
+                    for (int k = 0; k < V; ++k) v[e + p + k] = Elem<DT>::get(x[k]);
+                }
+                if (LIST) {
+#pragma unroll
+                    for (int p = 0; p < 8; p += 4) {
+                        const v4f x = *(const v4f*)(buf + (r0 + line) * sh.cols + c0 + at + e + p);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) m[e + p + k] = x[k];
+                    }
+                }
+            }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (row_in && c0 + at + e < sh.cols) {
+                v[e] = Elem<DT>::get(g[(r0 + line) * stride + c0 + at + e]);
+                if (LIST) m[e] = buf[(r0 + line) * sh.cols + c0 + at + e];
+            }
     }
+    const double sq = block_sum(t < nparts ? parts[(long long)mat * nparts + t] : 0.0, part);
+    const double inv = scale / (sqrt(sq) + eps);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        if (LIST) v[e] = src.nesterov ? v[e] + src.momentum * m[e] : m[e];
+        v[e] = (float)((double)v[e] * inv);
+        tile[line][at + e] = v[e];
+    }
+    auto put = [&](char* p, const float (&x)[16]) {
+        float a[8], b[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            a[e] = x[e];
+            b[e] = x[8 + e];
+        }
+        split8_put(p, a);
+        split8_put(p + 16, b);
+    };
+    if (row_in && c0 + at < ncp) put(nat + mat * nat_mat + split_at(r0 + line, ncp * 4, c0 + at), v);
+    __syncthreads();
     if (c0 + line < sh.cols && r0 + at < nrp) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) split_of(tile[at + e][line], hi.h[e], lo.h[e]);
-        char* p = tra + mat * tra_mat + split_at(c0 + line, nrp * 4, r0 + at);
-        *(v4i*)p = hi.w[0];
-        *(v4i*)(p + 16) = hi.w[1];
-        *(v4i*)(p + 64) = lo.w[0];
-        *(v4i*)(p + 80) = lo.w[1];
+        for (int e = 0; e < 16; ++e) v[e] = tile[at + e][line];
+        put(tra + mat * tra_mat + split_at(c0 + line, nrp * 4, r0 + at), v);
     }
 }
 
@@ -179,16 +276,6 @@ struct NsProducts {
     float* partial;
 };
 
-__device__ __forceinline__ float split_get(const char* p) {
-    return (float)*(const _Float16*)p + (float)*(const _Float16*)(p + 64);
-}
-__device__ __forceinline__ void split_put(char* p, float v) {
-    _Float16 hi, lo;
-    split_of(v, hi, lo);
-    *(_Float16*)p = hi;
-    *(_Float16*)(p + 64) = lo;
-}
-
 __device__ __forceinline__ void triangle(int t, int& i, int& j) {
     i = (int)((sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);
     while ((i + 1) * (i + 2) / 2 <= t) ++i;
@@ -196,25 +283,61 @@ __device__ __forceinline__ void triangle(int t, int& i, int& j) {
     j = t - i * (i + 1) / 2;
 }
 
-// four numbers (m, n .. n + 3) of a product
-__device__ __forceinline__ void ns_store_sym(const NsProduct& p, const NsProducts& a, long long mat, long long m, long long n,
-                                             const v4f& d) {
-    if (m >= a.lk || n >= a.l || n > m) return;
+// The wavefront's part of a tile: its rows from m0 and columns from n0 on, turned through LDS 16 rows at a time: eight
+// neighbours of a row to their place, eight neighbours of a column to the other side.  Of a tile on the diagonal only what
+// is on and below it is taken: both sides hold the same bits.  (They have to.  A product here takes the rows of its second
+// factor for columns, so what is not symmetric would enter the next step with its sign turned round, where it grows
+// by a - R = 6 instead of a + R = 0.7: two sides that differ in their last bit ended 2e-3 off.)
+template <class T>
+__device__ __forceinline__ void ns_store_sym(const NsProduct& p, const NsProducts& a, long long mat, long long m0, long long n0,
+                                             bool diagonal, LdsPtr turn, const typename T::Acc (&acc)[T::TM][T::TN]) {
     const long long ld = a.lk * 4;
     char* out = p.out + mat * p.out_mat;
+    const char* E1 = p.E1 ? p.E1 + mat * p.out_mat : nullptr;
+    const char* E2 = p.E2 ? p.E2 + mat * p.out_mat : nullptr;
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const long long c = n + r;
-        if (c >= a.l || c > m) continue;
-        float v = 0.0f;
-        if (m < a.l) {
-            const long long at = split_at(m, ld, c);
-            v = p.k0 * d[r];
-            if (p.E1) v += p.k1 * split_get(p.E1 + mat * p.out_mat + at);
-            if (p.E2) v += p.k2 * split_get(p.E2 + mat * p.out_mat + at);
-            split_put(out + at, v);
+    for (int i = 0; i < T::TM; ++i) {
+        float d[T::TN][4];
+#pragma unroll
+        for (int j = 0; j < T::TN; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) d[j][r] = p.k0 * acc[i][j][r];
+        turn_in<T::TN>(turn, d);
+        turn_out<T::TN, 8>(turn, [&](int row, int col, float (&v)[8]) {
+            const long long m = m0 + i * 16 + row, n = n0 + col;
+            const bool inside = m < a.l && n < a.lk;
+            const long long at = split_at(m, ld, n);
+            float e[8];
+            if (inside && E1) {
+                split_get_n<8>(E1 + at, e);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] += p.k1 * e[k];
+            }
+            if (inside && E2) {
+                split_get_n<8>(E2 + at, e);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] += p.k2 * e[k];
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (m >= a.l || n + k >= a.l) v[k] = 0.0f;      // zeros past the matrix
+            if (inside) split8_put_some(out + at, v, 0, diagonal ? m - n + 1 : 8);
+#pragma unroll
+            for (int k = 0; k < 8; k += 4)
+                *(__attribute__((address_space(3))) v4f*)(turn + row * TURN_LINE<T::TN> + (col + k) * 4) = v4f{v[k], v[k + 1], v[k + 2], v[k + 3]};
+        });
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int c = lane; c < T::TN * 32; c += 64) {        // (column, half of the 16 rows)
+            const int col = c % (T::TN * 16), half = c / (T::TN * 16) * 8;
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                v[k] = *(const __attribute__((address_space(3))) float*)(turn + (half + k) * TURN_LINE<T::TN> + col * 4);
+            const long long n = n0 + col, m = m0 + i * 16 + half;
+            if (n < a.l && m < a.lk) split8_put_some(out + split_at(n, ld, m), v, diagonal ? n - m + 1 : 0, 8);
         }
-        split_put(out + split_at(c, ld, m), v);      // the other side; zeros past the matrix
     }
 }
 
@@ -236,42 +359,43 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_product_kernel(NsProducts 
     const int k0 = slice * a.per_slice;
     const int k1 = k0 + a.per_slice < p.blocks ? k0 + a.per_slice : p.blocks;
     T::run(A, B, k0, k1, ring, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long m0 = (long long)ti * BM + (wave / WN) * (BM / WM) + piece_across(lane);
-    const long long n0 = (long long)tj * BM + (wave % WN) * (BM / WN) + piece_along(lane);
-    float* part = a.partial + id * (BM * BM) + threadIdx.x * 4;
+    const int wave = threadIdx.x >> 6;
+    if (a.slices > 1) {
+        float* part = a.partial + id * (BM * BM) + threadIdx.x * 4;
 #pragma unroll
-    for (int i = 0; i < T::TM; ++i)
+        for (int i = 0; i < T::TM; ++i)
 #pragma unroll
-        for (int j = 0; j < T::TN; ++j) {
-            if (a.slices == 1) ns_store_sym(p, a, mat, m0 + i * 16, n0 + j * 16, acc[i][j]);
-            else *(v4f*)(part + (i * T::TN + j) * T::THREADS * 4) = acc[i][j];
-        }
+            for (int j = 0; j < T::TN; ++j) *(v4f*)(part + (i * T::TN + j) * T::THREADS * 4) = acc[i][j];
+        return;
+    }
+    __syncthreads();
+    LdsPtr turn = (wave & 1 ? ring[1] : ring[0]) + (wave >> 1) * TURN_BYTES<T::TN>;
+    ns_store_sym<T>(p, a, mat, (long long)ti * BM + (wave / WN) * (BM / WM), (long long)tj * BM + (wave % WN) * (BM / WN), ti == tj,
+                    turn, acc);
 }
 
 // the slices of ns_product_kernel added in order, same geometry
 template <int BM, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(64 * WM * WN, 2) void ns_join_kernel(NsProducts a) {
     typedef TileProduct<MathSplit, BM, BM, WM, WN, STAGES, true> T;
+    __shared__ __align__(16) char lds[T::WAVES * TURN_BYTES<T::TN>];
     const NsProduct p = a.job[0];
     const long long per = (long long)a.tiles * a.count;
     const long long mt = blockIdx.x;
     const long long mat = mt / a.tiles;
     int ti, tj;
     triangle((int)(mt - mat * a.tiles), ti, tj);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long m0 = (long long)ti * BM + (wave / WN) * (BM / WM) + piece_across(lane);
-    const long long n0 = (long long)tj * BM + (wave % WN) * (BM / WN) + piece_along(lane);
+    const int wave = threadIdx.x >> 6;
     const float* part = a.partial + mt * (BM * BM) + threadIdx.x * 4;
+    typename T::Acc acc[T::TM][T::TN] = {};
+    for (int s = 0; s < a.slices; ++s)
 #pragma unroll
-    for (int i = 0; i < T::TM; ++i)
+        for (int i = 0; i < T::TM; ++i)
 #pragma unroll
-        for (int j = 0; j < T::TN; ++j) {
-            v4f d = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (int s = 0; s < a.slices; ++s)
-                d += *(const v4f*)(part + (long long)s * per * (BM * BM) + (i * T::TN + j) * T::THREADS * 4);
-            ns_store_sym(p, a, mat, m0 + i * 16, n0 + j * 16, d);
-        }
+            for (int j = 0; j < T::TN; ++j)
+                acc[i][j] += *(const v4f*)(part + (long long)s * per * (BM * BM) + (i * T::TN + j) * T::THREADS * 4);
+    ns_store_sym<T>(p, a, mat, (long long)ti * BM + (wave / WN) * (BM / WM), (long long)tj * BM + (wave % WN) * (BM / WN), ti == tj,
+                    (LdsPtr)lds + wave * TURN_BYTES<T::TN>, acc);
 }
 
 // ---------------------------------------------------------------- Y = q X + S X
@@ -285,7 +409,7 @@ struct NsApply {
     // NS_OUT_RESULT
     void* out;
     long long out_b, out_r;          // elements from matrix to matrix and row to row
-    int whole;                       // four neighbours of a row may be stored at once
+    int store;                       // how a row of the result, or of the weights, is stored
     // NS_OUT_WEIGHT
     void* param[NS_MAX_LIST];
     float decay, step;               // p = decay * p - step * Y
@@ -314,42 +438,73 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_apply_kernel(NsApply a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const char* x = TALL ? a.Xt + mat * a.xt_mat : a.X + mat * a.x_mat;
     const long long ldx = TALL ? ld : ldn;
-    const long long along_end = TALL ? sh.l : sh.n, across_end = TALL ? sh.n : sh.l, along_pad = TALL ? sh.lk : sh.nk;
+    const long long cols = TALL ? sh.l : sh.n, rows = TALL ? sh.n : sh.l, cols_pad = TALL ? sh.lk : sh.nk;
+    const long long mw = ti * BM + (wave / WN) * (BM / WM), nw = tj * BN + (wave % WN) * (BN / WN);
+    constexpr int ACROSS = TALL ? T::TN : T::TM, ALONG = TALL ? T::TM : T::TN;
+    static_assert((T::WAVES + 1) / 2 * TURN_BYTES<ALONG> <= T::HALF, "fits two stages");
+    __syncthreads();
+    LdsPtr turn = (wave & 1 ? ring[1] : ring[0]) + (wave >> 1) * TURN_BYTES<ALONG>;
 #pragma unroll
-    for (int i = 0; i < T::TM; ++i)
+    for (int i = 0; i < ACROSS; ++i) {
+        float d[ALONG][4];
 #pragma unroll
-        for (int j = 0; j < T::TN; ++j) {
-            const long long m = ti * BM + (wave / WN) * (BM / WM) + i * 16, n = tj * BN + (wave % WN) * (BN / WN) + j * 16;
-            const long long row = (TALL ? n : m) + piece_across(lane), col = (TALL ? m : n) + piece_along(lane);
-            if (OUT == NS_OUT_SPLIT && row >= across_end && row < sh.lk) {      // a row of X' ends in zeros
+        for (int j = 0; j < ALONG; ++j)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (col + r < along_end) split_put(a.Yt + mat * a.xt_mat + split_at(col + r, ld, row), 0.0f);
+            for (int r = 0; r < 4; ++r) d[j][r] = a.k0 * (TALL ? acc[j][i][r] : acc[i][j][r]);
+        turn_in<ALONG>(turn, d);
+        const long long r0 = (TALL ? nw : mw) + i * 16, c0 = TALL ? mw : nw;
+        // v += k1 * X; false where there is nothing
+        auto add = [&](long long row, long long col, auto& v) {
+            constexpr int W = (int)(sizeof(v) / sizeof(float));
+            if (row >= rows || col >= cols_pad) return false;
+            float e[W];
+            split_get_n<W>(x + split_at(row, ldx, col), e);
+#pragma unroll
+            for (int k = 0; k < W; ++k) v[k] += a.k1 * e[k];
+            return true;
+        };
+        if constexpr (OUT == NS_OUT_SPLIT) {
+            turn_out<ALONG, 8>(turn, [&](int r, int c, float (&v)[8]) {
+                const long long row = r0 + r, col = c0 + c;
+                const bool in = add(row, col, v);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = in && col + k < cols ? v[k] * a.again : 0.0f;
+                if (in) split8_put(a.Yn + mat * a.x_mat + split_at(row, ldn, col), v);
+#pragma unroll
+                for (int k = 0; k < 8; k += 4)
+                    *(__attribute__((address_space(3))) v4f*)(turn + r * TURN_LINE<ALONG> + (c + k) * 4) = v4f{v[k], v[k + 1], v[k + 2], v[k + 3]};
+            });
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int c = lane; c < ALONG * 32; c += 64) {        // rows of X', eight neighbours along l; they end in zeros
+                const int col = c % (ALONG * 16), half = c / (ALONG * 16) * 8;
+                float v[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    v[k] = *(const __attribute__((address_space(3))) float*)(turn + (half + k) * TURN_LINE<ALONG> + col * 4);
+                if (c0 + col < cols && r0 + half < sh.lk) split8_put(a.Yt + mat * a.xt_mat + split_at(c0 + col, ld, r0 + half), v);
             }
-            if (row >= across_end || col >= along_pad) continue;
-            const char* px = x + split_at(row, ldx, col);      // whole blocks of four: inside the padding
-            const v4h hi = *(const v4h*)px, lo = *(const v4h*)(px + 64);
-            float y[4];
+        } else {
+            auto emit = [&](int r, int c, auto& v) {
+                constexpr int W = (int)(sizeof(v) / sizeof(float));
+                const long long row = r0 + r, col = c0 + c;
+                if (!add(row, col, v)) return;
+                if constexpr (OUT == NS_OUT_RESULT) {
+                    put_row<DT, W>((E*)a.out + mat * a.out_b, row, col, rows, cols, a.out_r, v);
+                } else {
+                    E* p = (E*)a.param[mat];
+                    float w[W];
+                    get_row<DT, W>(p, row, col, cols, w);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) y[r] = a.k0 * acc[i][j][r] + a.k1 * ((float)hi[r] + (float)lo[r]);
-            const int left = along_end - col < 4 ? (int)(along_end - col) : 4;
-            if (OUT == NS_OUT_RESULT) {
-                if (left > 0) put4<DT>((E*)a.out + mat * a.out_b + row * a.out_r + col, y, left, a.whole);
-            } else if (OUT == NS_OUT_WEIGHT) {
-                E* p = (E*)a.param[mat] + row * along_end + col;
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (r < left) p[r] = Elem<DT>::put(a.decay * Elem<DT>::get(p[r]) - a.step * y[r]);
-            } else {
-                // !TALL here: rows of X along n, rows of X' along l
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float v = r < left ? y[r] * a.again : 0.0f;
-                    split_put(a.Yn + mat * a.x_mat + split_at(row, ldn, col + r), v);
-                    if (r < left) split_put(a.Yt + mat * a.xt_mat + split_at(col + r, ld, row), v);
+                    for (int k = 0; k < W; ++k) w[k] = a.decay * w[k] - a.step * v[k];
+                    put_row<DT, W>(p, row, col, rows, cols, cols, w);
                 }
-            }
+            };
+            if (a.store == STORE_16) turn_out<ALONG, 16 / (int)sizeof(E)>(turn, emit);
+            else if (sizeof(E) == 2 && a.store == STORE_PAIR) turn_out<ALONG, 2>(turn, emit);
+            else turn_out<ALONG, 1>(turn, emit);
         }
+    }
 }
 
 }  // namespace yh

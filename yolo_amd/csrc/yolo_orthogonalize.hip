@@ -19,8 +19,21 @@ inline int launch_status() {
 inline size_t dtype_bytes(int dt) { return dt == YH_F32 ? 4 : 2; }
 
 constexpr int64_t kMaxShort = 32768, kMaxLong = (int64_t)1 << 24, kMaxNumbers = (int64_t)1 << 38;
-constexpr int TB = 128;                       // tile of the products
-typedef TileProduct<MathSplit, TB, TB, 2, 4, 4, true> Tile;
+// Tiles of the products, as in the 8-bit product: us for a block of 32 numbers of the contraction with one workgroup on a
+// CU, and for each more that fits.  Square ones also serve the symmetric products.
+struct TileKind {
+    int bm, bn, per_cu;
+    double block, more;
+};
+constexpr int kKinds = 4;
+constexpr TileKind kTiles[kKinds] = {{256, 128, 1, 1.50, 0.0}, {128, 128, 1, 0.80, 0.0}, {64, 64, 2, 0.33, 0.20}, {32, 32, 5, 0.14, 0.09}};
+
+// us for `wgs` workgroups of `blocks` blocks each
+double tile_time(const TileKind& k, int64_t wgs, int64_t blocks) {
+    const int64_t at_once = 256 * (int64_t)k.per_cu;
+    const int64_t together = wgs >= at_once ? k.per_cu : (wgs + 255) / 256;
+    return (double)((wgs + at_once - 1) / at_once) * ((double)blocks * (k.block + k.more * (double)(together - 1)) + 3.0);
+}
 
 // powers of two the split matrices are held at: A and T up to about 1.5, R up to 127, S up to 1023
 constexpr float kScaleA = 512.0f, kScaleR = 512.0f, kScaleS = 64.0f, kScaleX = 4096.0f;
@@ -43,7 +56,7 @@ int check_sizes(int64_t count, int64_t rows, int64_t cols) {
     const int64_t l = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
     if (l > kMaxShort || n > kMaxLong || l * n > kMaxNumbers) return YH_ERR_SHAPE;
     // workgroups of a launch (256 threads each; a grid holds fewer than 2^32 threads)
-    if (count > kMaxNumbers / (l * n) || (count < 1 ? 1 : count) * ((l + 63) / 64) * ((n + 63) / 64) >= ((int64_t)1 << 24))
+    if (count > kMaxNumbers / (l * n) || (count < 1 ? 1 : count) * ((l + 31) / 32) * ((n + 31) / 32) >= ((int64_t)1 << 24))
         return YH_ERR_SHAPE;
     return YH_OK;
 }
@@ -51,8 +64,15 @@ int check_sizes(int64_t count, int64_t rows, int64_t cols) {
 struct Layout {
     size_t parts, x, xt, xt2, a, r0, r1, t, s0, s1, partial, total;
     long long x_mat, xt_mat, sq_mat;
-    int norm_blocks, tiles, slices, per_slice;
+    int norm_blocks;
+    int gram, tiles, slices, per_slice;      // X X': kind of tile, tiles on and below the diagonal, slices
+    int square, square_tiles;                // the l x l products
 };
+
+inline int triangle_tiles(int64_t l, int b) {
+    const int64_t side = (l + b - 1) / b;
+    return (int)(side * (side + 1) / 2);
+}
 
 Layout layout_for(const NsShape& s) {
     Layout w = {};
@@ -61,14 +81,32 @@ Layout layout_for(const NsShape& s) {
     w.x_mat = s.l * s.nk * 4;
     w.xt_mat = s.n * s.lk * 4;
     w.sq_mat = s.l * s.lk * 4;
-    const int64_t side = (s.l + TB - 1) / TB;
-    w.tiles = (int)(side * (side + 1) / 2);
     // the contraction of X X' is cut when the tiles alone do not fill the card
-    const int64_t blocks = s.nk / 32, wgs = (int64_t)w.tiles * s.count;
-    int64_t cut = wgs >= 256 ? 1 : (512 + wgs - 1) / wgs;
-    if (cut > (blocks + 7) / 8) cut = (blocks + 7) / 8;
-    w.per_slice = (int)((blocks + cut - 1) / cut);
-    w.slices = (int)((blocks + w.per_slice - 1) / w.per_slice);
+    const int64_t blocks = s.nk / 32;
+    double best = 0.0, best_square = 0.0;
+    for (int k = 1; k < kKinds; ++k) {
+        const int t = triangle_tiles(s.l, kTiles[k].bm);
+        const int64_t wgs = (int64_t)t * s.count;
+        for (int cut = 1; cut <= 16 && cut * 4 <= blocks + 3; cut *= 2) {
+            if (cut > 1 && wgs * cut > 2048) break;
+            const int64_t per = (blocks + cut - 1) / cut;
+            double us = tile_time(kTiles[k], wgs * cut, per);
+            if (cut > 1) us += 4.0 + (double)(wgs * (cut + 1)) * kTiles[k].bm * kTiles[k].bm * 4.0 / 3e6;
+            if (best == 0.0 || us < best) {
+                best = us;
+                w.gram = k;
+                w.tiles = t;
+                w.per_slice = (int)per;
+                w.slices = (int)((blocks + per - 1) / per);
+            }
+        }
+        const double us = tile_time(kTiles[k], wgs, s.lk / 32);
+        if (best_square == 0.0 || us < best_square) {
+            best_square = us;
+            w.square = k;
+            w.square_tiles = t;
+        }
+    }
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t at = off; off += up256(bytes); return at; };
     w.parts = take((size_t)s.count * w.norm_blocks * 8);
@@ -81,7 +119,7 @@ Layout layout_for(const NsShape& s) {
     w.t = take((size_t)s.count * w.sq_mat);
     w.s0 = take((size_t)s.count * w.sq_mat);
     w.s1 = take((size_t)s.count * w.sq_mat);
-    w.partial = take(w.slices > 1 ? (size_t)w.slices * w.tiles * s.count * TB * TB * 4 : 0);
+    w.partial = take(w.slices > 1 ? (size_t)w.slices * w.tiles * s.count * kTiles[w.gram].bm * kTiles[w.gram].bm * 4 : 0);
     w.total = off;
     return w;
 }
@@ -95,11 +133,28 @@ struct Sink {
     float decay, step;
 };
 
+template <int DT, int OUT, bool TALL, int BM, int BN, int WM, int WN, int STAGES>
+void apply_tiles(const NsApply& a, hipStream_t st) {
+    const int64_t tiles = ((a.sh.l + BM - 1) / BM) * ((a.sh.n + BN - 1) / BN) * a.sh.count;
+    hipLaunchKernelGGL((ns_apply_kernel<DT, OUT, TALL, BM, BN, WM, WN, STAGES>), dim3((unsigned)tiles), dim3(64 * WM * WN), 0, st, a);
+}
+
 template <int DT, int OUT, bool TALL>
 int apply(const NsApply& a, hipStream_t st) {
-    const int64_t tiles = ((a.sh.l + TB - 1) / TB) * ((a.sh.n + TB - 1) / TB) * a.sh.count;
-    hipLaunchKernelGGL((ns_apply_kernel<DT, OUT, TALL, TB, TB, 2, 4, 4>), dim3((unsigned)tiles), dim3(Tile::THREADS),
-                       0, st, a);
+    int kind = 0;
+    double best = 0.0;
+    for (int k = 0; k < kKinds; ++k) {
+        const int64_t wgs = ((a.sh.l + kTiles[k].bm - 1) / kTiles[k].bm) * ((a.sh.n + kTiles[k].bn - 1) / kTiles[k].bn) * a.sh.count;
+        const double us = tile_time(kTiles[k], wgs, a.sh.lk / 32);
+        if (best == 0.0 || us < best) {
+            best = us;
+            kind = k;
+        }
+    }
+    if (kind == 0) apply_tiles<DT, OUT, TALL, 256, 128, 4, 2, 3>(a, st);
+    else if (kind == 1) apply_tiles<DT, OUT, TALL, 128, 128, 2, 4, 4>(a, st);
+    else if (kind == 2) apply_tiles<DT, OUT, TALL, 64, 64, 2, 2, 4>(a, st);
+    else apply_tiles<DT, OUT, TALL, 32, 32, 2, 2, 4>(a, st);
     return launch_status();
 }
 
@@ -110,26 +165,37 @@ int apply_as(int dt, bool tall, const NsApply& a, hipStream_t st) {
     return tall ? apply<DT_BF16, OUT, true>(a, st) : apply<DT_BF16, OUT, false>(a, st);
 }
 
-int products(const NsProducts& a, int jobs, hipStream_t st) {
+template <int BM, int WM, int WN, int STAGES>
+int products_of(const NsProducts& a, int jobs, hipStream_t st) {
     const unsigned grid = (unsigned)((int64_t)a.tiles * a.count * a.slices);
-    hipLaunchKernelGGL((ns_product_kernel<TB, 2, 4, 4>), dim3(grid, (unsigned)jobs), dim3(Tile::THREADS), 0, st, a);
+    hipLaunchKernelGGL((ns_product_kernel<BM, WM, WN, STAGES>), dim3(grid, (unsigned)jobs), dim3(64 * WM * WN), 0, st, a);
     if (const int rc = launch_status()) return rc;
     if (a.slices > 1)
-        hipLaunchKernelGGL((ns_join_kernel<TB, 2, 4, 4>), dim3((unsigned)(a.tiles * a.count)), dim3(Tile::THREADS), 0, st, a);
+        hipLaunchKernelGGL((ns_join_kernel<BM, WM, WN, STAGES>), dim3((unsigned)(a.tiles * a.count)), dim3(64 * WM * WN), 0, st, a);
     return launch_status();
+}
+
+int products(int kind, const NsProducts& a, int jobs, hipStream_t st) {
+    if (kind == 1) return products_of<128, 2, 4, 4>(a, jobs, st);
+    if (kind == 2) return products_of<64, 2, 2, 4>(a, jobs, st);
+    return products_of<32, 2, 2, 4>(a, jobs, st);
 }
 
 template <int DT, bool LIST>
 int load(const NsSource& src, const NsShape& s, const Layout& w, char* ws, double eps, double scale, hipStream_t st) {
+    bool on16 = LIST || (aligned(src.base, 16) && src.stride_r % 8 == 0 && src.stride_b % 8 == 0);
+    if (LIST)
+        for (int i = 0; i < s.count; ++i) on16 = on16 && aligned(src.g[i], 16) && aligned(src.buf[i], 16);
+    const int vec = on16 && s.cols % 8 == 0;
     hipLaunchKernelGGL((ns_norm_kernel<DT, LIST>), dim3((unsigned)w.norm_blocks, (unsigned)s.count), dim3(256), 0, st, src, s,
-                       (double*)(ws + w.parts));
+                       (double*)(ws + w.parts), vec && (LIST || src.stride_r == s.cols));
     if (const int rc = launch_status()) return rc;
     char* x = ws + w.x;
     char* xt = ws + w.xt;
     hipLaunchKernelGGL((ns_convert_kernel<DT, LIST>),
                        dim3((unsigned)(((s.cols + 63) / 64) * ((s.rows + 63) / 64)), (unsigned)s.count), dim3(256), 0, st,
                        src, s, (const double*)(ws + w.parts), w.norm_blocks, eps, scale, s.tall ? xt : x,
-                       s.tall ? w.xt_mat : w.x_mat, s.tall ? x : xt, s.tall ? w.x_mat : w.xt_mat);
+                       s.tall ? w.xt_mat : w.x_mat, s.tall ? x : xt, s.tall ? w.x_mat : w.xt_mat, vec);
     return launch_status();
 }
 
@@ -151,7 +217,7 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, double scale, float a
     base.l = s.l;
     base.lk = s.lk;
     base.count = s.count;
-    base.tiles = w.tiles;
+    base.tiles = w.square_tiles;
     base.slices = 1;
     base.per_slice = lb;
     auto job = [&](const char* P, const char* Q, char* out, float k0, const char* E1, float k1, const char* E2, float k2) {
@@ -175,6 +241,7 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, double scale, float a
         for (double grown = fabs((double)a) * fabs((double)a); done + len < steps && grown <= limit; grown *= fabs((double)a)) ++len;
         // A = X X'
         NsProducts gram = base;
+        gram.tiles = w.tiles;
         gram.slices = w.slices;
         gram.per_slice = w.per_slice;
         gram.partial = (float*)(ws + w.partial);
@@ -182,7 +249,7 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, double scale, float a
         gram.job[0].p_mat = w.x_mat;
         gram.job[0].ldp = s.nk * 4;
         gram.job[0].blocks = (int)(s.nk / 32);
-        if (const int rc = products(gram, 1, st)) return rc;
+        if (const int rc = products(w.gram, gram, 1, st)) return rc;
         double q = a;                          // Q = q + S
         const char* Q = nullptr;
         float sq = 0.0f;
@@ -190,7 +257,7 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, double scale, float a
             char* Rj = R[j & 1];
             NsProducts one = base;
             one.job[0] = job(A, A, Rj, c * kScaleR / (kScaleA * kScaleA), A, b * kScaleR / kScaleA, nullptr, 0.0f);
-            if (const int rc = products(one, 1, st)) return rc;
+            if (const int rc = products(w.square, one, 1, st)) return rc;
             int jobs = 0;
             NsProducts two = base;
             const bool last = j + 1 == len;
@@ -205,11 +272,11 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, double scale, float a
                 sq = kScaleR;
             }
             if (jobs)
-                if (const int rc = products(two, jobs, st)) return rc;
+                if (const int rc = products(w.square, two, jobs, st)) return rc;
             if (!last) {
                 NsProducts three = base;
                 three.job[0] = job(T, Rj, A, 1.0f / kScaleR, T, a, nullptr, 0.0f);
-                if (const int rc = products(three, 1, st)) return rc;
+                if (const int rc = products(w.square, three, 1, st)) return rc;
             }
         }
         done += len;
@@ -233,7 +300,12 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, double scale, float a
             Xt_next = swap;
             scale = kScaleX;
         } else if (sink.params) {
-            for (int i = 0; i < s.count; ++i) ap.param[i] = sink.params[i];
+            bool on16 = (s.cols * (int64_t)dtype_bytes(sink.dtype)) % 16 == 0;
+            for (int i = 0; i < s.count; ++i) {
+                ap.param[i] = sink.params[i];
+                on16 = on16 && aligned(sink.params[i], 16);
+            }
+            ap.store = on16 ? STORE_16 : STORE_ONE;
             ap.decay = sink.decay;
             ap.step = sink.step;
             if (const int rc = apply_as<NS_OUT_WEIGHT>(sink.dtype, s.tall, ap, st)) return rc;
@@ -242,7 +314,9 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, double scale, float a
             ap.out_b = sink.out_b;
             ap.out_r = sink.out_r;
             const size_t e = dtype_bytes(sink.dtype);
-            ap.whole = aligned(sink.out, 4 * e) && sink.out_r % 4 == 0 && sink.out_b % 4 == 0;
+            if (aligned(sink.out, 16) && (sink.out_r * e) % 16 == 0 && (sink.out_b * e) % 16 == 0) ap.store = STORE_16;
+            else if (aligned(sink.out, 2 * e) && sink.out_r % 2 == 0 && sink.out_b % 2 == 0) ap.store = STORE_PAIR;
+            else ap.store = STORE_ONE;
             if (const int rc = apply_as<NS_OUT_RESULT>(sink.dtype, s.tall, ap, st)) return rc;
         }
     }
