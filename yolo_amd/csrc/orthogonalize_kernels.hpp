@@ -398,6 +398,175 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_join_kernel(NsProducts a) 
                     (LdsPtr)lds + wave * TURN_BYTES<T::TN>, acc);
 }
 
+// ---------------------------------------------------------------- a group of steps on a small A, in one launch
+// l <= SIDE: a workgroup per matrix runs the group from A to S.  The matrices stay in registers as fp32 (a wavefront owns a
+// block of T x T pieces on or below the diagonal), a product's two factors go through LDS in split form, written on both
+// sides of the diagonal from the one value below it.  13 to 17 products of which each as a launch of its own costs 3.5 us
+// take @CHAIN@.
+struct NsChain {
+    const char* A;
+    char* S;
+    long long mat;           // bytes from matrix to matrix of A and S
+    long long l, lk;
+    float a, b, c;
+    int steps;
+    float scale_a, scale_r, scale_s;     // of the matrices in LDS; A comes at scale_a, S leaves at scale_s (scale_r after one step)
+};
+
+template <int SIDE, int T>
+struct ChainGrid {
+    static constexpr int ROWS = SIDE / (16 * T), WAVES = ROWS * (ROWS + 1) / 2, THREADS = WAVES * 64;
+};
+
+template <int SIDE, int T>
+__global__ __launch_bounds__((ChainGrid<SIDE, T>::THREADS)) void ns_chain_kernel(NsChain p) {
+    constexpr int LINE = SIDE * 4, THREADS = ChainGrid<SIDE, T>::THREADS;
+    __shared__ __align__(1024) char left[SIDE * LINE], right[SIDE * LINE];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    int wi, wj;
+    triangle(wave, wi, wj);
+    const int m0 = wi * 16 * T + piece_across(lane), n0 = wj * 16 * T + piece_along(lane);     // of piece (0, 0)
+    const int l = (int)p.l;
+    typedef float Block[T][T][4];
+    auto at = [](int row, int col) {       // byte of hi in LDS; lo is the chunk four further on
+        const int chunk = (col & 31) >> 3;
+        return row * LINE + (col >> 5) * 128 + ((chunk ^ (row & 7)) << 4) + (col & 7) * 2;
+    };
+    auto lo_of = [](int at) { return at ^ 64; };
+    auto put = [&](char* to, const Block& v, float scale) {
+#pragma unroll
+        for (int i = 0; i < T; ++i)
+#pragma unroll
+            for (int j = 0; j < T; ++j) {
+                const int m = m0 + i * 16, n = n0 + j * 16;
+                _Float16 hi[4], lo[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) split_of(m < l && n + r < l ? v[i][j][r] * scale : 0.0f, hi[r], lo[r]);
+                if (n + 3 <= m) {
+                    const int q = at(m, n);
+                    *(v4h*)(to + q) = v4h{hi[0], hi[1], hi[2], hi[3]};
+                    *(v4h*)(to + lo_of(q)) = v4h{lo[0], lo[1], lo[2], lo[3]};
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (n + r <= m && n + 3 > m) {
+                        const int q = at(m, n + r);
+                        *(_Float16*)(to + q) = hi[r];
+                        *(_Float16*)(to + lo_of(q)) = lo[r];
+                    }
+                    if (n + r < m) {
+                        const int q = at(n + r, m);
+                        *(_Float16*)(to + q) = hi[r];
+                        *(_Float16*)(to + lo_of(q)) = lo[r];
+                    }
+                }
+            }
+    };
+    // out = k * (P Q'), this wavefront's block
+    auto product = [&](const char* P, const char* Q, float k, Block& out) {
+        v4f acc[T][T] = {};
+        const int lr = lane & 15, lq = lane >> 4;
+        const int c0 = (lq ^ (lr & 7)) << 4, c1 = ((4 + lq) ^ (lr & 7)) << 4;
+        const int pb = (wi * 16 * T + lr) * LINE, qb = (wj * 16 * T + lr) * LINE;
+#pragma unroll
+        for (int kb = 0; kb < SIDE / 32; ++kb) {
+            v4i fb[T][2];
+#pragma unroll
+            for (int j = 0; j < T; ++j) {
+                fb[j][0] = *(const v4i*)(Q + qb + j * 16 * LINE + kb * 128 + c0);
+                fb[j][1] = *(const v4i*)(Q + qb + j * 16 * LINE + kb * 128 + c1);
+            }
+#pragma unroll
+            for (int i = 0; i < T; ++i) {
+                v4i fa[2];
+                fa[0] = *(const v4i*)(P + pb + i * 16 * LINE + kb * 128 + c0);
+                fa[1] = *(const v4i*)(P + pb + i * 16 * LINE + kb * 128 + c1);
+                mma_row<MathSplit, true, 0, T>(acc[i], fa, fb);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < T; ++i)
+#pragma unroll
+            for (int j = 0; j < T; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) out[i][j][r] = k * acc[i][j][r];
+    };
+    auto mix = [&](Block& v, float x, const Block& u) {        // v += x * u
+#pragma unroll
+        for (int i = 0; i < T; ++i)
+#pragma unroll
+            for (int j = 0; j < T; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[i][j][r] += x * u[i][j][r];
+    };
+    Block A, R, X, S;
+    const char* ga = p.A + blockIdx.x * p.mat;
+    const long long ld = p.lk * 4;
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+#pragma unroll
+        for (int j = 0; j < T; ++j) {
+            const int m = m0 + i * 16, n = n0 + j * 16;
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (m < l && n < p.lk) split_get_n<4>(ga + split_at(m, ld, n), v);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) A[i][j][r] = v[r] / p.scale_a;
+        }
+    float q = p.a;
+    for (int step = 0; step < p.steps; ++step) {
+        const bool last = step + 1 == p.steps;
+        put(left, A, p.scale_a);
+        __syncthreads();
+        product(left, left, p.c / (p.scale_a * p.scale_a), R);
+        mix(R, p.b, A);
+        put(right, R, p.scale_r);
+        __syncthreads();
+        if (!last) {
+            product(right, left, 1.0f / (p.scale_r * p.scale_a), X);
+            mix(X, p.a, A);
+        }
+        if (step == 0) {
+#pragma unroll
+            for (int i = 0; i < T; ++i)
+#pragma unroll
+                for (int j = 0; j < T; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) S[i][j][r] = R[i][j][r];
+        } else {
+            __syncthreads();
+            put(left, S, p.scale_s);
+            __syncthreads();
+            Block N;
+            product(right, left, 1.0f / (p.scale_r * p.scale_s), N);
+            mix(N, p.a, S);
+            mix(N, q, R);
+            q *= p.a;
+#pragma unroll
+            for (int i = 0; i < T; ++i)
+#pragma unroll
+                for (int j = 0; j < T; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) S[i][j][r] = N[i][j][r];
+        }
+        __syncthreads();
+        if (!last) {
+            put(left, X, p.scale_a);
+            __syncthreads();
+            product(left, right, 1.0f / (p.scale_a * p.scale_r), A);
+            mix(A, p.a, X);
+            __syncthreads();
+        }
+    }
+    put(left, S, p.steps == 1 ? p.scale_r : p.scale_s);
+    __syncthreads();
+    char* gs = p.S + blockIdx.x * p.mat;
+    const int row_chunks = (int)(p.lk / 4);          // of 16 bytes
+    for (int i = t; i < l * row_chunks; i += THREADS) {
+        const int row = i / row_chunks, chunk = i - row * row_chunks;
+        *(v4i*)(gs + row * ld + chunk * 16) = *(const v4i*)(left + row * LINE + (chunk >> 3) * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+    }
+}
+
 // ---------------------------------------------------------------- Y = q X + S X
 enum { NS_OUT_RESULT = 0, NS_OUT_WEIGHT = 1, NS_OUT_SPLIT = 2 };
 

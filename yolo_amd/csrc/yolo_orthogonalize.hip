@@ -181,6 +181,16 @@ int products(int kind, const NsProducts& a, int jobs, hipStream_t st) {
     return products_of<32, 2, 2, 4>(a, jobs, st);
 }
 
+constexpr int kChainSide = 128;     // A up to this size is worked on by one workgroup
+
+int chain(const NsChain& c, int count, hipStream_t st) {
+    const dim3 grid((unsigned)count);
+    if (c.l <= 32) hipLaunchKernelGGL((ns_chain_kernel<32, 1>), grid, dim3(ChainGrid<32, 1>::THREADS), 0, st, c);
+    else if (c.l <= 64) hipLaunchKernelGGL((ns_chain_kernel<64, 1>), grid, dim3(ChainGrid<64, 1>::THREADS), 0, st, c);
+    else hipLaunchKernelGGL((ns_chain_kernel<128, 2>), grid, dim3(ChainGrid<128, 2>::THREADS), 0, st, c);
+    return launch_status();
+}
+
 template <int DT, bool LIST>
 int load(const NsSource& src, const NsShape& s, const Layout& w, char* ws, double eps, double scale, hipStream_t st) {
     bool on16 = LIST || (aligned(src.base, 16) && src.stride_r % 8 == 0 && src.stride_b % 8 == 0);
@@ -253,7 +263,25 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, double scale, float a
         double q = a;                          // Q = q + S
         const char* Q = nullptr;
         float sq = 0.0f;
-        for (int j = 0; j < len; ++j) {
+        if (s.l <= kChainSide) {
+            NsChain ch = {};
+            ch.A = A;
+            ch.S = S[0];
+            ch.mat = w.sq_mat;
+            ch.l = s.l;
+            ch.lk = s.lk;
+            ch.a = a;
+            ch.b = b;
+            ch.c = c;
+            ch.steps = len;
+            ch.scale_a = kScaleA;
+            ch.scale_r = kScaleR;
+            ch.scale_s = kScaleS;
+            if (const int rc = chain(ch, s.count, st)) return rc;
+            for (int j = 1; j < len; ++j) q *= a;
+            Q = S[0];
+            sq = len == 1 ? kScaleR : kScaleS;
+        } else for (int j = 0; j < len; ++j) {
             char* Rj = R[j & 1];
             NsProducts one = base;
             one.job[0] = job(A, A, Rj, c * kScaleR / (kScaleA * kScaleA), A, b * kScaleR / kScaleA, nullptr, 0.0f);
