@@ -34,7 +34,7 @@
 namespace yh {
 
 constexpr int NS_MAX_LIST = 32;      // matrices of one call that are handed over as a list of pointers
-constexpr int NS_NORM_BLOCKS = 256;  // partial sums of squares of a matrix, at most
+constexpr int NS_NORM_BLOCKS = 1024; // partial sums of squares of a matrix, at most
 
 // G: one strided batch, or a list of pointers
 struct NsSource {
@@ -230,7 +230,9 @@ __global__ __launch_bounds__(256) void ns_convert_kernel(NsSource src, NsShape s
                 if (LIST) m[e] = buf[(r0 + line) * sh.cols + c0 + at + e];
             }
     }
-    const double sq = block_sum(t < nparts ? parts[(long long)mat * nparts + t] : 0.0, part);
+    double some = 0.0;
+    for (int i = t; i < nparts; i += 256) some += parts[(long long)mat * nparts + i];
+    const double sq = block_sum(some, part);
     const double inv = scale / (sqrt(sq) + eps);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {

@@ -205,16 +205,17 @@ __device__ __forceinline__ void turn_in(LdsPtr turn, const float (&v)[PIECES][4]
 
 template <int PIECES, int WIDTH, class Emit>
 __device__ __forceinline__ void turn_out(LdsPtr turn, Emit&& emit) {
-    constexpr int PER_ROW = PIECES * 16 / WIDTH, ROWS = 64 / PER_ROW;
-    const int lane = threadIdx.x & 63, col = lane % PER_ROW * WIDTH;
+    constexpr int PER_ROW = PIECES * 16 / WIDTH, ITEMS = 16 * PER_ROW;
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int r0 = 0; r0 < 16; r0 += ROWS) {
-        const int row = r0 + lane / PER_ROW;
+    for (int base = 0; base < ITEMS; base += 64) {
+        const int item = base + lane, row = item / PER_ROW, col = item % PER_ROW * WIDTH;
+        if (ITEMS % 64 != 0 && item >= ITEMS) break;
         float v[WIDTH];
         if constexpr (WIDTH >= 4) {
 #pragma unroll
             for (int e = 0; e < WIDTH; e += 4) {
-                const v4f t = *(const __attribute__((address_space(3))) v4f*)(turn + (ROWS <= 16 ? row : row & 15) * TURN_LINE<PIECES> + (col + e) * 4);
+                const v4f t = *(const __attribute__((address_space(3))) v4f*)(turn + row * TURN_LINE<PIECES> + (col + e) * 4);
                 v[e] = t[0];
                 v[e + 1] = t[1];
                 v[e + 2] = t[2];
@@ -223,9 +224,9 @@ __device__ __forceinline__ void turn_out(LdsPtr turn, Emit&& emit) {
         } else {
 #pragma unroll
             for (int e = 0; e < WIDTH; ++e)
-                v[e] = *(const __attribute__((address_space(3))) float*)(turn + (ROWS <= 16 ? row : row & 15) * TURN_LINE<PIECES> + (col + e) * 4);
+                v[e] = *(const __attribute__((address_space(3))) float*)(turn + row * TURN_LINE<PIECES> + (col + e) * 4);
         }
-        if (ROWS <= 16 || row < 16) emit(row, col, v);
+        emit(row, col, v);
     }
 }
 

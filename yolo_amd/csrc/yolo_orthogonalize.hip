@@ -19,20 +19,24 @@ inline int launch_status() {
 inline size_t dtype_bytes(int dt) { return dt == YH_F32 ? 4 : 2; }
 
 constexpr int64_t kMaxShort = 32768, kMaxLong = (int64_t)1 << 24, kMaxNumbers = (int64_t)1 << 38;
-// Tiles of the products, as in the 8-bit product: us for a block of 32 numbers of the contraction with one workgroup on a
-// CU, and for each more that fits.  Square ones also serve the symmetric products.
+// Tiles of the products: us for a block of 32 numbers of the contraction with one workgroup on a CU, and for each more that
+// fits; `start` us to begin and end.  The square ones serve the symmetric products.  Measured there (us, 192 / 128 / 64 / 32;
+// l = contraction unless stated, matrices in brackets): 192 22 / 9.9 / 6.2 / 4.4, 512 (4) 31 / 15 / 8.9 / 8.6, 1024 44 / 22 / 12.1 /
+// 12.2, 1024 (4) 49 / 26 / 28 / 33, 1470 59 / 30 / 21 / 30, 2048 77 / 41 / 46 / 77, 4096 183 / 239 / 339 / -, 4096 over 50,176
+// 1974 / 2521 / 4531 / -: 4096 is 253 tiles of 192, one for each CU, but 528 of 128, two and a bit.
 struct TileKind {
     int bm, bn, per_cu;
-    double block, more;
+    double block, more, start;
 };
-constexpr int kKinds = 4;
-constexpr TileKind kTiles[kKinds] = {{256, 128, 1, 1.50, 0.0}, {128, 128, 1, 0.80, 0.0}, {64, 64, 2, 0.33, 0.20}, {32, 32, 5, 0.14, 0.09}};
+enum { TILE_256X128 = 0, TILE_192 = 1, TILE_128 = 2, TILE_64 = 3, TILE_32 = 4, TILE_KINDS = 5 };
+constexpr TileKind kTiles[TILE_KINDS] = {{256, 128, 1, 1.20, 0.0, 4.0}, {192, 192, 1, 1.30, 0.0, 6.0}, {128, 128, 1, 0.58, 0.0, 4.3},
+                                         {64, 64, 2, 0.23, 0.14, 4.3},  {32, 32, 5, 0.10, 0.11, 3.8}};
 
 // us for `wgs` workgroups of `blocks` blocks each
 double tile_time(const TileKind& k, int64_t wgs, int64_t blocks) {
     const int64_t at_once = 256 * (int64_t)k.per_cu;
     const int64_t together = wgs >= at_once ? k.per_cu : (wgs + 255) / 256;
-    return (double)((wgs + at_once - 1) / at_once) * ((double)blocks * (k.block + k.more * (double)(together - 1)) + 3.0);
+    return (double)((wgs + at_once - 1) / at_once) * ((double)blocks * (k.block + k.more * (double)(together - 1)) + k.start);
 }
 
 // powers of two the split matrices are held at: A and T up to about 1.5, R up to 127, S up to 1023
@@ -84,11 +88,11 @@ Layout layout_for(const NsShape& s) {
     // the contraction of X X' is cut when the tiles alone do not fill the card
     const int64_t blocks = s.nk / 32;
     double best = 0.0, best_square = 0.0;
-    for (int k = 1; k < kKinds; ++k) {
+    for (int k = TILE_192; k < TILE_KINDS; ++k) {
         const int t = triangle_tiles(s.l, kTiles[k].bm);
         const int64_t wgs = (int64_t)t * s.count;
         for (int cut = 1; cut <= 16 && cut * 4 <= blocks + 3; cut *= 2) {
-            if (cut > 1 && wgs * cut > 2048) break;
+            if (cut > 1 && wgs * cut > 4096) break;
             const int64_t per = (blocks + cut - 1) / cut;
             double us = tile_time(kTiles[k], wgs * cut, per);
             if (cut > 1) us += 4.0 + (double)(wgs * (cut + 1)) * kTiles[k].bm * kTiles[k].bm * 4.0 / 3e6;
@@ -143,7 +147,8 @@ template <int DT, int OUT, bool TALL>
 int apply(const NsApply& a, hipStream_t st) {
     int kind = 0;
     double best = 0.0;
-    for (int k = 0; k < kKinds; ++k) {
+    for (int k = 0; k <= TILE_32; ++k) {
+        if (k == TILE_192) continue;
         const int64_t wgs = ((a.sh.l + kTiles[k].bm - 1) / kTiles[k].bm) * ((a.sh.n + kTiles[k].bn - 1) / kTiles[k].bn) * a.sh.count;
         const double us = tile_time(kTiles[k], wgs, a.sh.lk / 32);
         if (best == 0.0 || us < best) {
@@ -151,9 +156,9 @@ int apply(const NsApply& a, hipStream_t st) {
             kind = k;
         }
     }
-    if (kind == 0) apply_tiles<DT, OUT, TALL, 256, 128, 4, 2, 3>(a, st);
-    else if (kind == 1) apply_tiles<DT, OUT, TALL, 128, 128, 2, 4, 4>(a, st);
-    else if (kind == 2) apply_tiles<DT, OUT, TALL, 64, 64, 2, 2, 4>(a, st);
+    if (kind == TILE_256X128) apply_tiles<DT, OUT, TALL, 256, 128, 4, 2, 3>(a, st);
+    else if (kind == TILE_128) apply_tiles<DT, OUT, TALL, 128, 128, 2, 4, 4>(a, st);
+    else if (kind == TILE_64) apply_tiles<DT, OUT, TALL, 64, 64, 2, 2, 4>(a, st);
     else apply_tiles<DT, OUT, TALL, 32, 32, 2, 2, 4>(a, st);
     return launch_status();
 }
@@ -176,8 +181,9 @@ int products_of(const NsProducts& a, int jobs, hipStream_t st) {
 }
 
 int products(int kind, const NsProducts& a, int jobs, hipStream_t st) {
-    if (kind == 1) return products_of<128, 2, 4, 4>(a, jobs, st);
-    if (kind == 2) return products_of<64, 2, 2, 4>(a, jobs, st);
+    if (kind == TILE_192) return products_of<192, 2, 4, 3>(a, jobs, st);
+    if (kind == TILE_128) return products_of<128, 2, 4, 4>(a, jobs, st);
+    if (kind == TILE_64) return products_of<64, 2, 2, 4>(a, jobs, st);
     return products_of<32, 2, 2, 4>(a, jobs, st);
 }
 
