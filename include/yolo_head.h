@@ -486,11 +486,12 @@ int yh_nms_ws(const float* cand_ltrb, const float* cand_score, const int32_t* ca
  * YH_MAX_I8_K), scales and bias are applied in fp32, the result is rounded once; bitwise
  * reproducible.  No gradient.
  * With YH_F32 and no bias y is the z of yh_decode_nms_linear.
- * workspace: yh_linear_i8_workspace_bytes bytes, 256-byte aligned, contents never matter.
+ * workspace: yh_linear_i8_workspace_bytes bytes, 256-byte aligned, contents never matter (NULL where
+ * it answers 0: a few rows are quantised on the way).
  */
 int yh_quantize_rows(const void* x, int x_dtype, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
                      int64_t rows, int64_t K, void* stream);
-size_t yh_linear_i8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+size_t yh_linear_i8_workspace_bytes(int x_dtype, int64_t M, int64_t N, int64_t K);
 int yh_linear_i8(const void* x, int x_dtype, int64_t ldx, const float* x_scale, const int8_t* w,
                  int64_t ldw, const float* w_scale, const float* bias, void* y, int y_dtype,
                  int64_t ldy, int64_t M, int64_t N, int64_t K, void* workspace,

@@ -132,6 +132,9 @@ def test_shapes_and_strides(dev):
     want = linear_i8(x.view(15, 96), w, t)
     assert torch.equal(linear_i8(x, w, t), want.view(3, 5, 40))
     assert torch.equal(linear_i8(x[1, 2], w, t), want[7])
+    odd = torch.empty(15 * 96 + 1, device=dev)[1:].view(15, 96)       # not on 16 bytes
+    odd.copy_(x.view(15, 96))
+    assert torch.equal(linear_i8(odd, w, t), want)
     wide = torch.randn(15, 203, generator=gen).to(dev)
     wide[:, 3:99] = x.view(15, 96)                                    # rows at an odd distance, not on 16 bytes
     assert torch.equal(linear_i8(wide[:, 3:99], w, t), want)
@@ -162,7 +165,7 @@ def test_what_lies_between_the_rows_of_y_stays(dev, m):
     w, t = weights(n, k, gen, dev)
     x = torch.randn(m, k, generator=gen).to(dev)
     y = torch.full((m + 1, ldy), 7.0, device=dev)
-    ws = torch.empty(lib.yh_linear_i8_workspace_bytes(m, n, k), dtype=torch.uint8, device=dev)
+    ws = torch.empty(lib.yh_linear_i8_workspace_bytes(_lib.YH_F32, m, n, k), dtype=torch.uint8, device=dev)
     _lib.check(lib.yh_linear_i8(x.data_ptr(), _lib.YH_F32, k, None, w.data_ptr(), w.stride(0), t.data_ptr(), None, y.data_ptr(),
                                 _lib.YH_F32, ldy, m, n, k, ws.data_ptr(), ws.numel(), torch.cuda.current_stream(dev).cuda_stream))
     assert torch.equal(y[:m, :n], linear_i8(x, w, t))

@@ -130,7 +130,7 @@ SIGNATURES = {
                           c_float, c_float, c_int64, c_int, c_void_p, c_size_t, c_void_p]),
     "yh_quantize_rows": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64,
                                  c_void_p]),
-    "yh_linear_i8_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "yh_linear_i8_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64]),
     "yh_linear_i8": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
                              c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_size_t,
                              c_void_p]),

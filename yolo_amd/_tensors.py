@@ -14,8 +14,8 @@ def _ptr(t: Optional[torch.Tensor]):
 def _stream(device) -> int:
     """The handle of the current stream of ``device`` (torch.cuda.current_stream builds an object around
     it, which costs several microseconds per call)."""
-    index = device.index if device.index is not None else torch.cuda.current_device()
-    return torch._C._cuda_getCurrentRawStream(index)
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 class _on_device:
@@ -25,8 +25,8 @@ class _on_device:
     __slots__ = ("ctx",)
 
     def __init__(self, device):
-        idx = device.index if device.index is not None else torch.cuda.current_device()
-        self.ctx = None if idx == torch.cuda.current_device() else torch.cuda.device(idx)
+        idx = device.index
+        self.ctx = None if idx is None or idx == torch.cuda.current_device() else torch.cuda.device(idx)
 
     def __enter__(self):
         if self.ctx is not None:
@@ -48,6 +48,6 @@ def _need(t: torch.Tensor, name: str, dtype, shape=None) -> torch.Tensor:
         raise ValueError(f"{name}: expected dtype {dtype}, got {t.dtype}")
     if not t.is_contiguous():
         raise ValueError(f"{name}: must be contiguous")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape and tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     return t

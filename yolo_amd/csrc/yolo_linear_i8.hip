@@ -119,6 +119,10 @@ constexpr int kRows = 16;      // rows linear_i8_rows_kernel takes
 // 8.0 / 7.8, 16 x 4096 14.2 / 8.9, 1 x 50,176 46.1 / 50.5); they have to fit its LDS.
 inline bool quantizes_itself(int64_t M, int64_t blocks) { return blocks <= 512 && (M == 1 || M * blocks <= 96); }
 
+inline size_t workspace_of(const Plan& p, int x_dtype, int64_t M) {
+    return x_dtype != YH_I8 && M <= kRows && quantizes_itself(M, p.blocks) ? 0 : p.total;
+}
+
 template <int DTX, int DT, bool QUANTIZE>
 int few_rows(const LinearI8Args& a, const void* x, int64_t ldx, int K, hipStream_t st) {
     hipLaunchKernelGGL((linear_i8_rows_kernel<DTX, DT, QUANTIZE>), dim3((unsigned)((a.N + 15) / 16)), dim3(1024),
@@ -178,9 +182,9 @@ int yh_quantize_rows(const void* x, int x_dtype, int64_t ldx, int8_t* q, int64_t
     return quantize(x, x_dtype, ldx, q, ldq, scale, nullptr, rows, (int)K, (int)Kz, (hipStream_t)stream);
 }
 
-size_t yh_linear_i8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+size_t yh_linear_i8_workspace_bytes(int x_dtype, int64_t M, int64_t N, int64_t K) {
     if (check_sizes(M, N, K) != YH_OK || M == 0 || N == 0) return 0;
-    return plan_for(M, N, K).total;
+    return workspace_of(plan_for(M, N, K), x_dtype, M);
 }
 
 int yh_linear_i8(const void* x, int x_dtype, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw,
@@ -193,7 +197,8 @@ int yh_linear_i8(const void* x, int x_dtype, int64_t ldx, const float* x_scale, 
     if (M == 0 || N == 0) return YH_OK;
     if (!x || !w || !w_scale || !y) return YH_ERR_NULL;
     const Plan p = plan_for(M, N, K);
-    if (!workspace || workspace_bytes < p.total) return YH_ERR_WORKSPACE;
+    const size_t need = workspace_of(p, x_dtype, M);
+    if (need && (!workspace || workspace_bytes < need)) return YH_ERR_WORKSPACE;
     if (!aligned(x, dtype_bytes(x_dtype)) || !aligned(x_scale, 4) || !aligned(w, 16) || ldw % 16 != 0 ||
         !aligned(w_scale, 4) || !aligned(bias, 4) || !aligned(y, dtype_bytes(y_dtype)) || !aligned(workspace, 256))
         return YH_ERR_ALIGN;
@@ -220,7 +225,7 @@ int yh_linear_i8(const void* x, int x_dtype, int64_t ldx, const float* x_scale, 
     a.tiles_n = p.tiles_n;
     const size_t e = dtype_bytes(y_dtype);
     a.store = (ldy * e) % 16 == 0 && aligned(y, 16) ? STORE_16 : ldy % 2 == 0 && aligned(y, 2 * e) ? STORE_PAIR : STORE_ONE;
-    if (x_dtype != YH_I8 && M <= kRows && quantizes_itself(M, p.blocks)) {
+    if (need == 0) {
         if (y_dtype == YH_F32) return few_rows_of<DT_F32>(a, x, x_dtype, ldx, (int)K, st);
         if (y_dtype == YH_F16) return few_rows_of<DT_F16>(a, x, x_dtype, ldx, (int)K, st);
         return few_rows_of<DT_BF16>(a, x, x_dtype, ldx, (int)K, st);

@@ -21,8 +21,8 @@ _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
 @lru_cache(maxsize=4096)
-def _workspace_bytes(m: int, n: int, k: int) -> int:
-    return _lib.load().yh_linear_i8_workspace_bytes(m, n, k)
+def _workspace_bytes(code: int, m: int, n: int, k: int) -> int:
+    return _lib.load().yh_linear_i8_workspace_bytes(code, m, n, k)
 
 
 def _no_grad(t: torch.Tensor, name: str) -> None:
@@ -41,7 +41,8 @@ def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
         raise ValueError(f"{name}: expected shape (..., K) with K in 1 .. {_lib.YH_MAX_I8_K}, got {tuple(x.shape)}")
     if x.stride(-1) != 1 and x.shape[-1] > 1:
         raise ValueError(f"{name}: must be contiguous along its last axis")
-    x = x.detach()
+    if x.requires_grad:
+        x = x.detach()
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1]) if x.numel() else x.new_empty(0, x.shape[-1])
     if x.shape[0] > 1 and x.stride(0) < x.shape[1]:      # expanded or overlapping rows
@@ -88,9 +89,10 @@ def linear_i8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
     x = _rows(x, "x")
     m, k = x.shape
     dev = x.device
-    if x.dtype not in _lib.DTYPE_CODES:
+    code = _lib.DTYPE_CODES.get(x.dtype)
+    if code is None:
         raise ValueError(f"x: expected dtype float32, float16, bfloat16 or int8, got {x.dtype}")
-    if (x.dtype == torch.int8) != (x_scale is not None):
+    if (code == _lib.YH_I8) != (x_scale is not None):
         raise ValueError("x_scale: the scales of an int8 x, and of nothing else")
     if x_scale is not None:
         _need(x_scale, "x_scale", torch.float32)
@@ -99,30 +101,32 @@ def linear_i8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.shape[1] != k or weight.dtype != torch.int8:
         raise ValueError(f"weight: expected an int8 tensor of shape (N, {k})")
     n = weight.shape[0]
-    ldw = weight.stride(0) if n > 1 else (k + 15) // 16 * 16
-    end = weight.storage_offset() + (n - 1) * ldw + (k + 15) // 16 * 16
-    if n and ((weight.stride(1) != 1 and k > 1) or ldw < k or ldw % 16 or weight.data_ptr() % 16
-              or end > weight.untyped_storage().nbytes()):
+    room = (k + 15) // 16 * 16
+    ldw, along = weight.stride()
+    ldw = ldw if n > 1 else room
+    if n and ((along != 1 and k > 1) or ldw < k or ldw % 16 or weight.data_ptr() % 16
+              or weight.storage_offset() + (n - 1) * ldw + room > weight.untyped_storage().nbytes()):
         raise ValueError("weight: unit stride along K, rows a multiple of 16 bytes apart and 16-byte aligned, the last one "
                          "with room up to the next multiple of 16 bytes (quantize_rows lays it out so)")
     _need(weight_scale, "weight_scale", torch.float32, (n,))
     if bias is not None:
-        bias = _need(bias.detach(), "bias", torch.float32, (n,))
+        _need(bias, "bias", torch.float32, (n,))
     for name, t in (("weight", weight), ("weight_scale", weight_scale), ("bias", bias), ("x_scale", x_scale)):
         if t is not None and t.device != dev:
             raise ValueError(f"{name}: on {t.device}, x is on {dev}")
     if out_dtype is None:
-        out_dtype = torch.float32 if x.dtype == torch.int8 else x.dtype
+        out_dtype = torch.float32 if code == _lib.YH_I8 else x.dtype
     if out_dtype not in _FLOATS:
         raise ValueError(f"out_dtype: expected float32, float16 or bfloat16, got {out_dtype}")
-    y = torch.empty(*shape[:-1], n, dtype=out_dtype, device=dev)
-    if y.numel() == 0:
+    y = torch.empty((*shape[:-1], n), dtype=out_dtype, device=dev)
+    if m == 0 or n == 0:
         return y
-    ws = torch.empty(_workspace_bytes(m, n, k), dtype=torch.uint8, device=dev)
+    nbytes = _workspace_bytes(code, m, n, k)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with _on_device(dev):
-        _lib.check(_lib.load().yh_linear_i8(x.data_ptr(), _lib.DTYPE_CODES[x.dtype], _ld(x), _ptr(x_scale), weight.data_ptr(), ldw,
-                                    weight_scale.data_ptr(), _ptr(bias), y.data_ptr(), _lib.DTYPE_CODES[out_dtype], n, m, n,
-                                    k, ws.data_ptr(), ws.numel(), _stream(dev)))
+        _lib.check(_lib.load().yh_linear_i8(
+            x.data_ptr(), code, _ld(x), _ptr(x_scale), weight.data_ptr(), ldw, weight_scale.data_ptr(), _ptr(bias),
+            y.data_ptr(), _lib.DTYPE_CODES[out_dtype], n, m, n, k, _ptr(ws), nbytes, _stream(dev)))
     return y
 
 
