@@ -13,8 +13,8 @@ BIG = 1 << 40
 
 
 def _linear(**kw):
-    a = dict(x=FAKE, xd=_lib.YH_F32, ldx=64, sx=None, w=FAKE, ldw=64, sw=FAKE, bias=None, y=FAKE, yd=_lib.YH_F32, ldy=8,
-             M=40, N=8, K=64, ws=FAKE, nbytes=BIG)
+    a = dict(x=FAKE, xd=_lib.YH_F32, ldx=64, sx=None, w=FAKE, ldw=64, sw=FAKE, bias=None, y=FAKE, yd=_lib.YH_F32, ldy=800,
+             M=600, N=800, K=64, ws=FAKE, nbytes=BIG)
     a.update(kw)
     return _lib.load().yh_linear_i8(a["x"], a["xd"], a["ldx"], a["sx"], a["w"], a["ldw"], a["sw"], a["bias"], a["y"], a["yd"],
                                     a["ldy"], a["M"], a["N"], a["K"], a["ws"], a["nbytes"], None)
@@ -27,7 +27,7 @@ def _linear(**kw):
     (dict(M=1 << 22), _lib.YH_ERR_SHAPE),
     (dict(ldx=63), _lib.YH_ERR_SHAPE),
     (dict(ldw=48), _lib.YH_ERR_SHAPE),
-    (dict(ldy=7), _lib.YH_ERR_SHAPE),
+    (dict(ldy=799), _lib.YH_ERR_SHAPE),
     (dict(xd=4), _lib.YH_ERR_ARG),
     (dict(yd=_lib.YH_I8), _lib.YH_ERR_ARG),
     (dict(sx=FAKE), _lib.YH_ERR_ARG),                    # scales for an x that is not int8
@@ -98,9 +98,9 @@ def test_muon_step_argument_errors(kw, rc):
 def test_workspace_sizes():
     lib = _lib.load()
     assert lib.yh_linear_i8_workspace_bytes(_lib.YH_F32, 0, 8, 64) == 0 and lib.yh_linear_i8_workspace_bytes(_lib.YH_F32, 4, 8, 0) == 0
-    assert lib.yh_linear_i8_workspace_bytes(_lib.YH_I8, 3, 8, 200) >= 3 * 256 + 3 * 4
+    assert lib.yh_linear_i8_workspace_bytes(_lib.YH_I8, 600, 800, 200) >= 600 * 256
     assert lib.yh_linear_i8_workspace_bytes(_lib.YH_F32, 3, 8, 200) == 0          # quantised on the way
-    assert lib.yh_linear_i8_workspace_bytes(_lib.YH_F32, 30, 8, 200) >= 30 * 256 + 30 * 4
+    assert lib.yh_linear_i8_workspace_bytes(_lib.YH_F32, 30, 8, 4096) >= 30 * 4096 + 30 * 4
     assert lib.yh_orthogonalize_workspace_bytes(0, 8, 8) == 0 and lib.yh_orthogonalize_workspace_bytes(1, 0, 8) == 0
     assert lib.yh_orthogonalize_workspace_bytes(1, 64, 147) == lib.yh_orthogonalize_workspace_bytes(1, 147, 64) > 0
 

@@ -34,6 +34,9 @@ template <> struct Elem<DT_F16> {
     static __device__ __forceinline__ float get(T v) { return (float)v; }
     static __device__ __forceinline__ T put(float f) { return (_Float16)f; }
 };
+template <> struct Elem<DT_I8> {
+    using T = int8_t;
+};
 template <> struct Elem<DT_BF16> {
     using T = unsigned short;
     static __device__ __forceinline__ float get(T v) { return bf16_to_f32(v); }
@@ -108,8 +111,12 @@ __device__ __forceinline__ void load16(const typename Elem<DT>::T* row, int i, i
             for (int e = 0; e < V; ++e) f[p * V + e] = Elem<DT>::get(v[e]);
         }
     } else {
+        // every load is issued (the last number again past the end): loads behind conditions wait for each other
+        T v[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) f[e] = i + e < K ? Elem<DT>::get(row[i + e]) : 0.0f;
+        for (int e = 0; e < 16; ++e) v[e] = row[i + e < K ? i + e : K - 1];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) f[e] = i + e < K ? Elem<DT>::get(v[e]) : 0.0f;
     }
 }
 
@@ -396,28 +403,28 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_i8_tile_kernel(LinearI
 }
 
 // the slices' sums (integers: any order gives the same), scales, bias
-// Up to 16 rows: the weight is read once, straight into registers, and that is what bounds it.  A workgroup of 16
-// wavefronts takes 16 channels; a wavefront takes every 16th block of 128 bytes of their rows, four blocks (8 KB) on
-// their way while four are worked on; the 16 sums meet in LDS.  QUANTIZE: the rows of x are quantised by every
-// workgroup for itself, into LDS, while its first weights are on their way: that costs less than a launch up to
-// 65,536 numbers, which is what a workgroup holds.  @ROWS@
-template <int DTX, int DT, bool QUANTIZE>
+// Up to 16 rows a workgroup (blockIdx.y: which): the weight is read once, straight into registers, and that is what bounds
+// it.  A workgroup of 16 wavefronts takes 16 channels; a wavefront takes every 16th block of 128 bytes of their rows, four
+// blocks (8 KB) on their way while four are worked on; the 16 sums meet in LDS.  STAGE: every workgroup brings the rows of x
+// into LDS for itself, quantised where they are not 8-bit already and padded with zeros, while its first weights are on
+// their way: for few rows that is less than a launch of its own.  Otherwise a.q holds the padded rows.  @ROWS@
+template <int DTX, int DT, bool STAGE>
 __global__ __launch_bounds__(1024) void linear_i8_rows_kernel(LinearI8Args a, const typename Elem<DTX>::T* __restrict__ x,
                                                               long long ldx, int K, int vec) {
     typedef typename Elem<DTX>::T T;
     constexpr int AHEAD = 4, WAVES = 16;
-    extern __shared__ __align__(16) char rows_lds[];        // QUANTIZE: M rows of a.blocks * 128 bytes
+    extern __shared__ __align__(16) char rows_lds[];        // STAGE: the rows, a.blocks * 128 bytes each
     __shared__ __align__(16) v4i sums[WAVES][64];
     __shared__ unsigned part[WAVES];
     __shared__ float row_s[16];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int lr = lane & 15, lq = (lane >> 4) * 16;
-    const long long n0 = (long long)blockIdx.x * 16;
-    const int M = (int)a.M;
+    const long long n0 = (long long)blockIdx.x * 16, m0 = (long long)blockIdx.y * 16;
+    const int M = a.M - m0 < 16 ? (int)(a.M - m0) : 16;
     const char* w = (const char*)a.w + (n0 + lr < a.N ? n0 + lr : a.N - 1) * a.ldw;
     const int m = lr < M ? lr : M - 1;
     const int row_bytes = a.blocks * 128;
-    const char* q = (const char*)a.q + m * a.ldq;
+    const char* q = (const char*)a.q + (m0 + m) * a.ldq;
     const int last = a.blocks - 1;
     v4i wr[2][AHEAD][2];
     auto fetch = [&](v4i (&r)[AHEAD][2], int kb) {
@@ -432,42 +439,60 @@ __global__ __launch_bounds__(1024) void linear_i8_rows_kernel(LinearI8Args a, co
             }
     };
     fetch(wr[0], wave);
-    if (QUANTIZE) {
+    if constexpr (STAGE) {
         // 1024 / rows threads (rounded down to a power of two) to a row, 16 numbers at a time
         int per = 1024;
         while (per * M > 1024) per >>= 1;
         const int row = t / per, at0 = (t & (per - 1)) * 16;
         const bool mine = row < M;
-        const T* xr = x + (mine ? row : 0) * ldx;
-        unsigned top = 0;
+        const T* xr = x + (m0 + (mine ? row : 0)) * ldx;
         const int end = mine ? K : 0, pad = mine ? row_bytes : 0;
-#pragma unroll 4
-        for (int i = at0; i < end; i += per * 16) {
-            float f[16];
-            load16<DTX>(xr, i, K, vec, f);
+        if constexpr (DTX == DT_I8) {
+            if (mine && at0 == 0) row_s[row] = a.sx[m0 + row];
+            for (int i = at0; i < pad; i += per * 16) {
+                Quantized o;
+                if (vec && i + 16 <= end) {
+                    o.w = *(const v4i*)(xr + i);
+                } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) top = max(top, magnitude(f[e]));
-        }
+                    for (int e = 0; e < 16; ++e) o.b[e] = i + e < end ? xr[i + e] : (int8_t)0;
+                }
+                *(v4i*)(rows_lds + row * row_bytes + i) = o.w;
+            }
+        } else {
+            unsigned top = 0;
+            float held[16];                              // short rows are read once
+            const bool once = K <= per * 16;
+            load16<DTX>(xr, mine ? at0 : K, K, vec, held);
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
-        if (lane == 0) part[wave] = top;
-        __syncthreads();
-        const int span = per / 64, first = (wave / span) * span;      // per is 64 at least: M <= 16
-        for (int i = 0; i < span; ++i) top = max(top, part[first + i]);
-        const float amax = __uint_as_float(top);
-        const bool finite = top < 0x7f800000u;
-        const double inv = finite && top ? 127.0 / (double)amax : 0.0;
-        if (mine && at0 == 0) row_s[row] = finite ? amax / 127.0f : __uint_as_float(0x7fc00000u);
+            for (int e = 0; e < 16; ++e) top = max(top, magnitude(held[e]));
 #pragma unroll 4
-        for (int i = at0; i < pad; i += per * 16) {
-            Quantized o;
-            o.w = v4i{0, 0, 0, 0};
-            if (inv > 0.0) {
+            for (int i = at0 + per * 16; i < end; i += per * 16) {
                 float f[16];
                 load16<DTX>(xr, i, K, vec, f);
-                quantize_some(f, inv, o.b);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = max(top, magnitude(f[e]));
             }
-            *(v4i*)(rows_lds + row * row_bytes + i) = o.w;
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
+            if (lane == 0) part[wave] = top;
+            __syncthreads();
+            const int span = per / 64, first = (wave / span) * span;      // per is 64 at least: M <= 16
+            for (int i = 0; i < span; ++i) top = max(top, part[first + i]);
+            const float amax = __uint_as_float(top);
+            const bool finite = top < 0x7f800000u;
+            const double inv = finite && top ? 127.0 / (double)amax : 0.0;
+            if (mine && at0 == 0) row_s[row] = finite ? amax / 127.0f : __uint_as_float(0x7fc00000u);
+#pragma unroll 4
+            for (int i = at0; i < pad; i += per * 16) {
+                Quantized o;
+                o.w = v4i{0, 0, 0, 0};
+                if (inv > 0.0) {
+                    if (!once) load16<DTX>(xr, i, K, vec, held);
+                    quantize_some(held, inv, o.b);
+                }
+                *(v4i*)(rows_lds + row * row_bytes + i) = o.w;
+            }
         }
         __syncthreads();
     }
@@ -480,7 +505,7 @@ __global__ __launch_bounds__(1024) void linear_i8_rows_kernel(LinearI8Args a, co
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int off = b * 128 + h * 64 + lq;
-                xr[u][h] = *(const v4i*)(QUANTIZE ? rows_lds + m * row_bytes + off : q + off);
+                xr[u][h] = *(const v4i*)(STAGE ? rows_lds + m * row_bytes + off : q + off);
             }
         }
 #pragma unroll
@@ -504,8 +529,8 @@ __global__ __launch_bounds__(1024) void linear_i8_rows_kernel(LinearI8Args a, co
         for (int i = 1; i < WAVES; ++i) d += sums[i][lane];
         if (lr < M) {
             LinearI8Args b = a;
-            if (QUANTIZE) b.sx = row_s;
-            linear_store<DT>(b, lr, n0 + piece_along(lane), d);
+            if (STAGE) b.sx = row_s - m0;
+            linear_store<DT>(b, m0 + lr, n0 + piece_along(lane), d);
         }
     }
 }

@@ -114,29 +114,35 @@ Plan plan_for(int64_t M, int64_t N, int64_t K) {
     return p;
 }
 
-constexpr int kRows = 16;      // rows linear_i8_rows_kernel takes
-// It quantises them itself when that is less than a launch by itself (us, with / without: 1 x 4096 5.7 / 7.1, 4 x 4096
-// 8.0 / 7.8, 16 x 4096 14.2 / 8.9, 1 x 50,176 46.1 / 50.5); they have to fit its LDS.
-inline bool quantizes_itself(int64_t M, int64_t blocks) { return blocks <= 512 && (M == 1 || M * blocks <= 96); }
-
-inline size_t workspace_of(const Plan& p, int x_dtype, int64_t M) {
-    return x_dtype != YH_I8 && M <= kRows && quantizes_itself(M, p.blocks) ? 0 : p.total;
+constexpr int kRows = 16;      // rows of a workgroup of linear_i8_rows_kernel
+// It brings the rows into LDS itself when that is less than a launch by itself (us, with / without: 1 x 4096 5.7 / 7.1, 4 x 4096
+// 8.0 / 7.8, 16 x 4096 14.2 / 8.9, 1 x 50,176 46.1 / 50.5): up to 12,288 numbers or one row (8-bit rows, which are only
+// copied: 65,536 bytes), and one workgroup a CU (64 x 700 -> 1470, 368 workgroups: 19.8 / 8.1).
+inline bool stages_itself(int x_dtype, int64_t M, int64_t N, int64_t blocks) {
+    const int64_t rows = M < kRows ? M : kRows;
+    if (((M + kRows - 1) / kRows) * ((N + 15) / 16) > 256) return M <= kRows && M * blocks <= 96;
+    return x_dtype == YH_I8 ? rows * blocks <= 512 && M <= kRows : blocks <= 512 && (M == 1 || rows * blocks <= 96);
+}
+inline size_t workspace_of(const Plan& p, int x_dtype, int64_t M, int64_t N) {
+    return stages_itself(x_dtype, M, N, p.blocks) ? 0 : p.total;
 }
 
-template <int DTX, int DT, bool QUANTIZE>
+template <int DTX, int DT, bool STAGE>
 int few_rows(const LinearI8Args& a, const void* x, int64_t ldx, int K, hipStream_t st) {
-    hipLaunchKernelGGL((linear_i8_rows_kernel<DTX, DT, QUANTIZE>), dim3((unsigned)((a.N + 15) / 16)), dim3(1024),
-                       QUANTIZE ? (size_t)a.M * a.blocks * 128 : 0, st, a, (const typename Elem<DTX>::T*)x, ldx, K,
-                       aligned(x, 16) && (a.M == 1 || (ldx * sizeof(typename Elem<DTX>::T)) % 16 == 0));
+    const int64_t rows = a.M < kRows ? a.M : kRows;
+    const int vec = aligned(x, 16) && (a.M == 1 || (ldx * sizeof(typename Elem<DTX>::T)) % 16 == 0);
+    hipLaunchKernelGGL((linear_i8_rows_kernel<DTX, DT, STAGE>), dim3((unsigned)((a.N + 15) / 16), (unsigned)((a.M + kRows - 1) / kRows)),
+                       dim3(1024), STAGE ? (size_t)rows * a.blocks * 128 : 0, st, a, (const typename Elem<DTX>::T*)x, ldx, K, vec);
     return launch_status();
 }
 
 template <int DT>
 int few_rows_of(const LinearI8Args& a, const void* x, int x_dtype, int64_t ldx, int K, hipStream_t st) {
+    if (!x) return few_rows<DT_I8, DT, false>(a, nullptr, 0, K, st);      // a.q holds the rows
     if (x_dtype == YH_F32) return few_rows<DT_F32, DT, true>(a, x, ldx, K, st);
     if (x_dtype == YH_F16) return few_rows<DT_F16, DT, true>(a, x, ldx, K, st);
     if (x_dtype == YH_BF16) return few_rows<DT_BF16, DT, true>(a, x, ldx, K, st);
-    return few_rows<DT_F32, DT, false>(a, nullptr, 0, K, st);      // a.q holds the rows
+    return few_rows<DT_I8, DT, true>(a, x, ldx, K, st);
 }
 
 template <int DT, int BM, int BN, int WM, int WN, int STAGES>
@@ -184,7 +190,7 @@ int yh_quantize_rows(const void* x, int x_dtype, int64_t ldx, int8_t* q, int64_t
 
 size_t yh_linear_i8_workspace_bytes(int x_dtype, int64_t M, int64_t N, int64_t K) {
     if (check_sizes(M, N, K) != YH_OK || M == 0 || N == 0) return 0;
-    return workspace_of(plan_for(M, N, K), x_dtype, M);
+    return workspace_of(plan_for(M, N, K), x_dtype, M, N);
 }
 
 int yh_linear_i8(const void* x, int x_dtype, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw,
@@ -197,7 +203,7 @@ int yh_linear_i8(const void* x, int x_dtype, int64_t ldx, const float* x_scale, 
     if (M == 0 || N == 0) return YH_OK;
     if (!x || !w || !w_scale || !y) return YH_ERR_NULL;
     const Plan p = plan_for(M, N, K);
-    const size_t need = workspace_of(p, x_dtype, M);
+    const size_t need = workspace_of(p, x_dtype, M, N);
     if (need && (!workspace || workspace_bytes < need)) return YH_ERR_WORKSPACE;
     if (!aligned(x, dtype_bytes(x_dtype)) || !aligned(x_scale, 4) || !aligned(w, 16) || ldw % 16 != 0 ||
         !aligned(w_scale, 4) || !aligned(bias, 4) || !aligned(y, dtype_bytes(y_dtype)) || !aligned(workspace, 256))
@@ -226,6 +232,7 @@ int yh_linear_i8(const void* x, int x_dtype, int64_t ldx, const float* x_scale, 
     const size_t e = dtype_bytes(y_dtype);
     a.store = (ldy * e) % 16 == 0 && aligned(y, 16) ? STORE_16 : ldy % 2 == 0 && aligned(y, 2 * e) ? STORE_PAIR : STORE_ONE;
     if (need == 0) {
+        a.sx = x_scale;
         if (y_dtype == YH_F32) return few_rows_of<DT_F32>(a, x, x_dtype, ldx, (int)K, st);
         if (y_dtype == YH_F16) return few_rows_of<DT_F16>(a, x, x_dtype, ldx, (int)K, st);
         return few_rows_of<DT_BF16>(a, x, x_dtype, ldx, (int)K, st);
