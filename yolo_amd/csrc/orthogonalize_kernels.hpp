@@ -434,33 +434,46 @@ __global__ __launch_bounds__((ChainGrid<SIDE, T>::THREADS)) void ns_chain_kernel
         const int chunk = (col & 31) >> 3;
         return row * LINE + (col >> 5) * 128 + ((chunk ^ (row & 7)) << 4) + (col & 7) * 2;
     };
-    auto lo_of = [](int at) { return at ^ 64; };
+    auto four = [](char* to, int q, const unsigned (&w)[4]) {        // words of hi (low half) and lo to two places of 8 bytes
+        typedef unsigned v2u __attribute__((ext_vector_type(2)));
+        *(v2u*)(to + q) = v2u{__builtin_amdgcn_perm(w[1], w[0], 0x05040100u), __builtin_amdgcn_perm(w[3], w[2], 0x05040100u)};
+        *(v2u*)(to + (q ^ 64)) = v2u{__builtin_amdgcn_perm(w[1], w[0], 0x07060302u), __builtin_amdgcn_perm(w[3], w[2], 0x07060302u)};
+    };
+    // A lane's four neighbours of a row go to their place at once; four lanes of neighbouring rows exchange theirs (a 4x4
+    // transposition, the lane one further, then the lane two further) and write four neighbours of a column to the other side.
     auto put = [&](char* to, const Block& v, float scale) {
+        const bool odd = lane & 1, high = lane & 2;
 #pragma unroll
         for (int i = 0; i < T; ++i)
 #pragma unroll
             for (int j = 0; j < T; ++j) {
-                const int m = m0 + i * 16, n = n0 + j * 16;
-                _Float16 hi[4], lo[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) split_of(m < l && n + r < l ? v[i][j][r] * scale : 0.0f, hi[r], lo[r]);
-                if (n + 3 <= m) {
-                    const int q = at(m, n);
-                    *(v4h*)(to + q) = v4h{hi[0], hi[1], hi[2], hi[3]};
-                    *(v4h*)(to + lo_of(q)) = v4h{lo[0], lo[1], lo[2], lo[3]};
-                }
+                const int m = m0 + i * 16, n = n0 + j * 16, mq = m & ~3;
+                unsigned d[4], x[4], c[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    if (n + r <= m && n + 3 > m) {
-                        const int q = at(m, n + r);
-                        *(_Float16*)(to + q) = hi[r];
-                        *(_Float16*)(to + lo_of(q)) = lo[r];
-                    }
-                    if (n + r < m) {
-                        const int q = at(n + r, m);
-                        *(_Float16*)(to + q) = hi[r];
-                        *(_Float16*)(to + lo_of(q)) = lo[r];
-                    }
+                    _Float16 hi, lo;
+                    split_of(m < l && n + r < l ? v[i][j][r] * scale : 0.0f, hi, lo);
+                    d[r] = (unsigned)__builtin_bit_cast(unsigned short, hi) | (unsigned)__builtin_bit_cast(unsigned short, lo) << 16;
+                }
+#pragma unroll
+                for (int r = 0; r < 4; r += 2) {
+                    const unsigned got = (unsigned)__builtin_amdgcn_mov_dpp((int)(odd ? d[r] : d[r + 1]), 0xB1, 0xF, 0xF, true);
+                    x[r] = odd ? got : d[r];
+                    x[r + 1] = odd ? d[r + 1] : got;
+                }
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const unsigned got = (unsigned)__builtin_amdgcn_mov_dpp((int)(high ? x[r] : x[r + 2]), 0x4E, 0xF, 0xF, true);
+                    c[r] = high ? got : x[r];
+                    c[r + 2] = high ? x[r + 2] : got;
+                }
+                if (n < mq) {
+                    four(to, at(m, n), d);
+                    four(to, at(n + (m & 3), mq), c);
+                } else if (n == mq) {                 // the 4x4 block on the diagonal: each side from below it
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) d[r] = r <= (m & 3) ? d[r] : c[r];
+                    four(to, at(m, n), d);
                 }
             }
     };

@@ -193,6 +193,7 @@ int chain(const NsChain& c, int count, hipStream_t st) {
     const dim3 grid((unsigned)count);
     if (c.l <= 32) hipLaunchKernelGGL((ns_chain_kernel<32, 1>), grid, dim3(ChainGrid<32, 1>::THREADS), 0, st, c);
     else if (c.l <= 64) hipLaunchKernelGGL((ns_chain_kernel<64, 1>), grid, dim3(ChainGrid<64, 1>::THREADS), 0, st, c);
+    else if (c.l <= 96) hipLaunchKernelGGL((ns_chain_kernel<96, 2>), grid, dim3(ChainGrid<96, 2>::THREADS), 0, st, c);
     else hipLaunchKernelGGL((ns_chain_kernel<128, 2>), grid, dim3(ChainGrid<128, 2>::THREADS), 0, st, c);
     return launch_status();
 }
