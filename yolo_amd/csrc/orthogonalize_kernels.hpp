@@ -77,7 +77,8 @@ __device__ __forceinline__ double block_sum(double v, double* part) {
 // ---------------------------------------------------------------- norm (and momentum)
 // Squares are added in 64 bits: no gradient in fp32 range overflows or vanishes.  One partial sum per workgroup, added
 // in order by whoever needs the norm: the same bits from run to run.  vec: matrices without gaps between rows, on 16 bytes
-// and of a multiple of eight numbers; a thread then takes eight at a time.  @NORM@
+// and of a multiple of eight numbers; a thread then takes eight at a time.  411 MB of bf16: 85 us (4.8 TB/s);
+// with momentum (38 M numbers, 375 MB): 62 us.
 template <int DT, bool LIST>
 __global__ __launch_bounds__(256) void ns_norm_kernel(NsSource src, NsShape sh, double* __restrict__ parts, int vec) {
     __shared__ double part[4];
@@ -181,7 +182,8 @@ __device__ __forceinline__ void split_get_n(const char* p, float (&v)[N]) {
 
 // ---------------------------------------------------------------- G -> X and X', split
 // 64 x 64 numbers of G per workgroup; `nat` gets G's own rows, `tra` its columns, both times scale / (|G| + eps).  vec: rows
-// of G (and of the momentum) on 16 bytes and of a multiple of eight numbers.  @CONVERT@
+// of G (and of the momentum) on 16 bytes and of a multiple of eight numbers.  4096 x 50,176 bf16: 518 us for 2.06 GB
+// (4.0 TB/s).
 template <int DT, bool LIST>
 __global__ __launch_bounds__(256) void ns_convert_kernel(NsSource src, NsShape sh, const double* __restrict__ parts, int nparts,
                                                          double eps, double scale, char* __restrict__ nat, long long nat_mat,
@@ -404,7 +406,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_join_kernel(NsProducts a) 
 // l <= SIDE: a workgroup per matrix runs the group from A to S.  The matrices stay in registers as fp32 (a wavefront owns a
 // block of T x T pieces on or below the diagonal), a product's two factors go through LDS in split form, written on both
 // sides of the diagonal from the one value below it.  13 to 17 products of which each as a launch of its own costs 3.5 us
-// take @CHAIN@.
+// take 9 us (30 rows), 16 us (64), 35 us (90), 53 us (128); LDS reads and the split writes share that time.
 struct NsChain {
     const char* A;
     char* S;
