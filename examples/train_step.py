@@ -6,9 +6,11 @@ feeding the HIP head.  The call shape is the reference's training loop
 (train.py:84-94): ``loss = model.get_loss(image, ...)``; ``loss.backward()``;
 ``optim.step()``.
 
-    python examples/train_step.py [--batch 8] [--steps 5] [--width 1.0]
+    python examples/train_step.py [--batch 8] [--steps 5] [--width 1.0] [--optim adamw|muon] [--int8]
 
-``--width`` scales the channel counts (0.25 gives a backbone that fits a quick test).
+``--width`` scales the channel counts (0.25 gives a backbone that fits a quick test).  ``--optim muon``
+steps the weight matrices by orthogonalised updates (``yolo_amd.Muon``) and the biases by AdamW;
+``--int8`` serves the last layer in 8-bit integers for the detections printed at the end.
 """
 from __future__ import annotations
 
@@ -21,7 +23,7 @@ import torch
 from torch import nn
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
-from yolo_amd import YOLOv1Head, synth  # noqa: E402
+from yolo_amd import Int8Linear, Muon, YOLOv1Head, synth  # noqa: E402
 
 # (out_channels, kernel, stride) or "M" for a 2x2 max-pool -- YOLOv1 paper, Fig. 3
 LAYERS = [(64, 7, 2), "M", (192, 3, 1), "M", (128, 1, 1), (256, 3, 1), (256, 1, 1), (512, 3, 1), "M",
@@ -46,31 +48,50 @@ def make_backbone(width: float = 1.0, n_cells: int = 7, depth: int = 30, hidden:
     return nn.Sequential(*mods)
 
 
-def main():
+def make_optimizers(net: nn.Module, kind: str):
+    """The optimizers of one step: AdamW over everything (train.py:84-94's), or Muon over the
+    weight matrices with AdamW over the rest."""
+    if kind == "adamw":
+        return [torch.optim.AdamW(net.parameters(), lr=1e-4)]
+    weights = [p for p in net.parameters() if p.dim() >= 2]
+    rest = [p for p in net.parameters() if p.dim() < 2]
+    return [Muon(weights, lr=2e-3, weight_decay=0.01), torch.optim.AdamW(rest, lr=1e-4)]
+
+
+def main(argv=None):
     ap = argparse.ArgumentParser()
     ap.add_argument("--batch", type=int, default=8)
     ap.add_argument("--steps", type=int, default=5)
     ap.add_argument("--width", type=float, default=1.0)
-    args = ap.parse_args()
+    ap.add_argument("--optim", choices=("adamw", "muon"), default="adamw")
+    ap.add_argument("--int8", action="store_true")
+    args = ap.parse_args(argv)
     dev = torch.device("cuda:0")
     torch.manual_seed(0)
     net = make_backbone(args.width).to(dev)
     head = YOLOv1Head(backbone=net)
-    optim = torch.optim.AdamW(net.parameters(), lr=1e-4)
+    optims = make_optimizers(net, args.optim)
     image = torch.randn(args.batch, 3, 448, 448, device=dev)
     _, gx, gc, om = (t.to(dev) for t in synth.make_inputs(args.batch, seed=0))
     for step in range(args.steps):
         torch.cuda.synchronize()
         t0 = time.perf_counter()
         loss = head.get_loss(image, gx, gc, om)           # train.py:84
-        optim.zero_grad()
+        for optim in optims:
+            optim.zero_grad()
         loss.backward()                                   # train.py:93
-        optim.step()
+        for optim in optims:
+            optim.step()
         torch.cuda.synchronize()
         dt = time.perf_counter() - t0
         c, f, k = head.last_loss_terms[:3].tolist()
         print(f"step {step}: loss {loss.item():.4f}  (coord {c:.1f}, conf {f:.1f}, cls {k:.1f})  {1e3 * dt:.1f} ms")
-    dets, count = head.postprocess(head(image).detach(), 0.5, 0.5)
+    with torch.no_grad():
+        if args.int8:
+            features = net.eval()[:-1](image)
+            dets, count = head.postprocess_linear(features, Int8Linear.from_linear(net[-1]), 0.5, 0.5)
+        else:
+            dets, count = head.postprocess(head(image), 0.5, 0.5)
     print("detections kept per image:", count.tolist())
 
 

@@ -99,6 +99,12 @@ def test_scale_zeros_and_what_is_not_a_number(dev):
     for power in (-100, -60, 60, 100):      # squares below and above the range of fp32 (entries stay inside it)
         # the norm, added in 64 bits, is the same number but for its power of two
         assert torch.equal(orthogonalize(g * 2.0 ** power, eps=0.0, out_dtype=torch.float32), want), power
+    # norms around and far below eps: X is small and stays so, to its last bits
+    for power, steps in ((-20, 5), (-30, 5), (-40, 5), (-60, 5), (-100, 5), (-30, 8), (-45, 8)):
+        small = g * 2.0 ** power
+        got = orthogonalize(small, steps=steps, out_dtype=torch.float32)
+        assert off(got, polar(small.cpu(), steps)) <= 1e-4, (power, steps)
+        assert off(orthogonalize(small, steps=steps), polar(small.cpu(), steps)) <= FAR[torch.bfloat16], (power, steps)
     batch = torch.stack([g, torch.zeros_like(g), g, g, g])
     batch[2, 17, 3] = float("nan")
     batch[3, 0, 0] = float("inf")
@@ -237,6 +243,25 @@ def test_optimizer(dev):
     optim.zero_grad()
     optim.step()                                          # no gradients: nothing moves
     assert torch.equal(frozen, weights[0].detach())
+
+
+def test_training_example(dev, capsys, monkeypatch):
+    """examples/train_step.py with orthogonalised updates and the last layer in 8 bits runs; its gradients are finite and
+    reach every weight."""
+    import os
+    import sys
+
+    monkeypatch.syspath_prepend(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples"))
+    train_step = __import__("train_step")
+    made = []
+    make = train_step.make_backbone
+    monkeypatch.setattr(train_step, "make_backbone", lambda *a, **k: made.append(make(*a, **k)) or made[-1])
+    train_step.main(["--batch", "2", "--steps", "2", "--width", "0.125", "--optim", "muon", "--int8"])
+    assert "detections kept per image" in capsys.readouterr().out
+    for name, p in made[0].named_parameters():
+        assert p.grad is not None and torch.isfinite(p.grad).all() and torch.isfinite(p).all(), name
+        assert p.grad.any(), name
+    sys.modules.pop("train_step", None)
 
 
 def test_training_step_of_the_head(dev):

@@ -22,6 +22,9 @@
 // arithmetic gives.  The entry points form a new A when a^steps would pass 64 (fp32 results) or 512 (16-bit
 // results, whose own rounding is 2e-3).
 //
+// X is held as a matrix of Frobenius norm `scale` and the factor |G| / (|G| + eps) / scale beside it, a number of its own for
+// each matrix: a gradient far below eps keeps its bits.
+//
 // A matrix of this file, "split": rows of 128-byte blocks, 32 numbers each, 64 bytes of hi and 64 bytes of lo, times
 // a power of two that keeps lo out of the subnormal range; zeros fill a row's last block.
 #pragma once
@@ -181,13 +184,13 @@ __device__ __forceinline__ void split_get_n(const char* p, float (&v)[N]) {
 }
 
 // ---------------------------------------------------------------- G -> X and X', split
-// 64 x 64 numbers of G per workgroup; `nat` gets G's own rows, `tra` its columns, both times scale / (|G| + eps).  vec: rows
+// 64 x 64 numbers of G per workgroup; `nat` gets G's own rows, `tra` its columns, both times scale / |G|.  vec: rows
 // of G (and of the momentum) on 16 bytes and of a multiple of eight numbers.  4096 x 50,176 bf16: 518 us for 2.06 GB
 // (4.0 TB/s).
 template <int DT, bool LIST>
 __global__ __launch_bounds__(256) void ns_convert_kernel(NsSource src, NsShape sh, const double* __restrict__ parts, int nparts,
                                                          double eps, double scale, char* __restrict__ nat, long long nat_mat,
-                                                         char* __restrict__ tra, long long tra_mat, int vec) {
+                                                         char* __restrict__ tra, long long tra_mat, float* __restrict__ factor, int vec) {
     typedef typename Elem<DT>::T T;
     __shared__ float tile[64][65];
     __shared__ double part[4];
@@ -235,7 +238,8 @@ __global__ __launch_bounds__(256) void ns_convert_kernel(NsSource src, NsShape s
     double some = 0.0;
     for (int i = t; i < nparts; i += 256) some += parts[(long long)mat * nparts + i];
     const double sq = block_sum(some, part);
-    const double inv = scale / (sqrt(sq) + eps);
+    const double norm = sqrt(sq), inv = norm == 0.0 ? 0.0 : scale / norm;
+    if (blockIdx.x == 0 && t == 0) factor[mat] = norm == 0.0 ? 0.0f : (float)(norm / (norm + eps) / scale);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
         if (LIST) v[e] = src.nesterov ? v[e] + src.momentum * m[e] : m[e];
@@ -269,6 +273,7 @@ struct NsProduct {
     char* out;
     long long p_mat, out_mat;       // bytes from matrix to matrix of P and Q; of E1, E2 and out
     long long ldp;                  // bytes from row to row of P and Q; lk * 4 in E1, E2 and out
+    const float* factor;            // of each matrix, or null: k0 times its square
     float k0, k1, k2;
     int blocks;                     // of 32 numbers along the contraction
 };
@@ -300,13 +305,14 @@ __device__ __forceinline__ void ns_store_sym(const NsProduct& p, const NsProduct
     const char* E1 = p.E1 ? p.E1 + mat * p.out_mat : nullptr;
     const char* E2 = p.E2 ? p.E2 + mat * p.out_mat : nullptr;
     const int lane = threadIdx.x & 63;
+    const float k0 = p.factor ? p.k0 * p.factor[mat] * p.factor[mat] : p.k0;
 #pragma unroll
     for (int i = 0; i < T::TM; ++i) {
         float d[T::TN][4];
 #pragma unroll
         for (int j = 0; j < T::TN; ++j)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) d[j][r] = p.k0 * acc[i][j][r];
+            for (int r = 0; r < 4; ++r) d[j][r] = k0 * acc[i][j][r];
         turn_in<T::TN>(turn, d);
         turn_out<T::TN, 8>(turn, [&](int row, int col, float (&v)[8]) {
             const long long m = m0 + i * 16 + row, n = n0 + col;
@@ -591,6 +597,7 @@ struct NsApply {
     const char *S, *X, *Xt;
     long long s_mat, x_mat, xt_mat;
     NsShape sh;
+    const float* factor;             // of each matrix: Y times it, where it leaves (NS_OUT_SPLIT keeps it apart)
     float k0, k1;                    // Y = k0 * (S X) + k1 * X
     // NS_OUT_RESULT
     void* out;
@@ -599,9 +606,8 @@ struct NsApply {
     // NS_OUT_WEIGHT
     void* param[NS_MAX_LIST];
     float decay, step;               // p = decay * p - step * Y
-    // NS_OUT_SPLIT: Y times `again`
+    // NS_OUT_SPLIT
     char *Yn, *Yt;
-    float again;
 };
 
 template <int DT, int OUT, bool TALL, int BM, int BN, int WM, int WN, int STAGES>
@@ -630,13 +636,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_apply_kernel(NsApply a) {
     static_assert((T::WAVES + 1) / 2 * TURN_BYTES<ALONG> <= T::HALF, "fits two stages");
     __syncthreads();
     LdsPtr turn = (wave & 1 ? ring[1] : ring[0]) + (wave >> 1) * TURN_BYTES<ALONG>;
+    const float factor = OUT == NS_OUT_SPLIT ? 1.0f : a.factor[mat];
+    const float k0 = a.k0 * factor, k1 = a.k1 * factor;
 #pragma unroll
     for (int i = 0; i < ACROSS; ++i) {
         float d[ALONG][4];
 #pragma unroll
         for (int j = 0; j < ALONG; ++j)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) d[j][r] = a.k0 * (TALL ? acc[j][i][r] : acc[i][j][r]);
+            for (int r = 0; r < 4; ++r) d[j][r] = k0 * (TALL ? acc[j][i][r] : acc[i][j][r]);
         turn_in<ALONG>(turn, d);
         const long long r0 = (TALL ? nw : mw) + i * 16, c0 = TALL ? mw : nw;
         // v += k1 * X; false where there is nothing
@@ -646,7 +654,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_apply_kernel(NsApply a) {
             float e[W];
             split_get_n<W>(x + split_at(row, ldx, col), e);
 #pragma unroll
-            for (int k = 0; k < W; ++k) v[k] += a.k1 * e[k];
+            for (int k = 0; k < W; ++k) v[k] += k1 * e[k];
             return true;
         };
         if constexpr (OUT == NS_OUT_SPLIT) {
@@ -654,7 +662,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_apply_kernel(NsApply a) {
                 const long long row = r0 + r, col = c0 + c;
                 const bool in = add(row, col, v);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = in && col + k < cols ? v[k] * a.again : 0.0f;
+                for (int k = 0; k < 8; ++k)
+                    if (!in || col + k >= cols) v[k] = 0.0f;
                 if (in) split8_put(a.Yn + mat * a.x_mat + split_at(row, ldn, col), v);
 #pragma unroll
                 for (int k = 0; k < 8; k += 4)

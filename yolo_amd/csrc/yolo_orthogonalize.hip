@@ -46,7 +46,7 @@ double tile_time(const TileKind& k, int64_t wgs, int64_t blocks) {
 }
 
 // powers of two the split matrices are held at: A and T up to about 1.5, R up to 127, S up to 1023
-constexpr float kScaleA = 512.0f, kScaleR = 512.0f, kScaleS = 64.0f, kScaleX = 4096.0f;
+constexpr float kScaleA = 512.0f, kScaleR = 512.0f, kScaleS = 64.0f;
 
 NsShape shape_of(int64_t rows, int64_t cols, int count) {
     NsShape s = {};
@@ -72,7 +72,7 @@ int check_sizes(int64_t count, int64_t rows, int64_t cols) {
 }
 
 struct Layout {
-    size_t parts, x, xt, xt2, a, r0, r1, t, s0, s1, partial, total;
+    size_t parts, factor, x, xt, xt2, a, r0, r1, t, s0, s1, partial, total;
     long long x_mat, xt_mat, sq_mat;
     int norm_blocks;
     int gram, tiles, slices, per_slice;      // X X': kind of tile, tiles on and below the diagonal, slices
@@ -120,6 +120,7 @@ Layout layout_for(const NsShape& s) {
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t at = off; off += up256(bytes); return at; };
     w.parts = take((size_t)s.count * w.norm_blocks * 8);
+    w.factor = take((size_t)s.count * 4);
     w.x = take((size_t)s.count * w.x_mat);
     w.xt = take((size_t)s.count * w.xt_mat);
     w.xt2 = take((size_t)s.count * w.xt_mat);
@@ -218,7 +219,7 @@ int load(const NsSource& src, const NsShape& s, const Layout& w, char* ws, doubl
     hipLaunchKernelGGL((ns_convert_kernel<DT, LIST>),
                        dim3((unsigned)(((s.cols + 63) / 64) * ((s.rows + 63) / 64)), (unsigned)s.count), dim3(256), 0, st,
                        src, s, (const double*)(ws + w.parts), w.norm_blocks, eps, scale, s.tall ? xt : x,
-                       s.tall ? w.xt_mat : w.x_mat, s.tall ? x : xt, s.tall ? w.x_mat : w.xt_mat, vec);
+                       s.tall ? w.xt_mat : w.x_mat, s.tall ? x : xt, s.tall ? w.x_mat : w.xt_mat, (float*)(ws + w.factor), vec);
     return launch_status();
 }
 
@@ -229,12 +230,14 @@ int load_as(int dt, const NsSource& src, const NsShape& s, const Layout& w, char
     return load<DT_BF16, LIST>(src, s, w, ws, eps, scale, st);
 }
 
-// G is in the workspace as X and X' (at `scale`); the steps, and the result to `sink`
+// G is in the workspace as X and X' (of norm `scale`, their factor beside them); the steps, and the result to `sink`
 int run_steps(const NsShape& s, const Layout& w, char* ws, double scale, float a, float b, float c, int steps, const Sink& sink,
               hipStream_t st) {
     char *A = ws + w.a, *T = ws + w.t, *R[2] = {ws + w.r0, ws + w.r1}, *S[2] = {ws + w.s0, ws + w.s1};
     char *X = ws + w.x, *Xt = ws + w.xt, *Xt_next = ws + w.xt2;
     const int lb = (int)(s.lk / 32);
+    const float* factor = (const float*)(ws + w.factor);
+    double rest = 1.0, held = scale;           // X_j = rest * factor * (what is held), which has grown from norm `held`
     const double limit = sink.dtype == YH_F32 ? 64.0 : 512.0;
     NsProducts base = {};
     base.l = s.l;
@@ -268,7 +271,8 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, double scale, float a
         gram.slices = w.slices;
         gram.per_slice = w.per_slice;
         gram.partial = (float*)(ws + w.partial);
-        gram.job[0] = job(X, X, A, (float)(kScaleA / (scale * scale)), nullptr, 0.0f, nullptr, 0.0f);
+        gram.job[0] = job(X, X, A, (float)(kScaleA * rest * rest), nullptr, 0.0f, nullptr, 0.0f);
+        gram.job[0].factor = factor;
         gram.job[0].p_mat = w.x_mat;
         gram.job[0].ldp = s.nk * 4;
         gram.job[0].blocks = (int)(s.nk / 32);
@@ -329,17 +333,22 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, double scale, float a
         ap.x_mat = w.x_mat;
         ap.xt_mat = w.xt_mat;
         ap.sh = s;
-        ap.k0 = (float)(1.0 / (sq * scale));
-        ap.k1 = (float)(q / scale);
+        // what is held next: as large as the growth of `done` steps leaves room for below fp16's largest number
+        double next = ldexp(1.0, (int)floor(log2(32768.0 / pow(fabs((double)a) < 1.0 ? 1.0 : fabs((double)a), (double)done))));
+        if (next < 1.0) next = 1.0;
+        const double k = done < steps ? next / held : rest;
+        ap.factor = factor;
+        ap.k0 = (float)(k / sq);
+        ap.k1 = (float)(k * q);
         if (done < steps) {
             ap.Yn = X;
             ap.Yt = Xt_next;
-            ap.again = kScaleX;
             if (const int rc = apply<DT_F32, NS_OUT_SPLIT, false>(ap, st)) return rc;
             char* swap = Xt;
             Xt = Xt_next;
             Xt_next = swap;
-            scale = kScaleX;
+            rest *= held / next;
+            held = next;
         } else if (sink.params) {
             bool on16 = (s.cols * (int64_t)dtype_bytes(sink.dtype)) % 16 == 0;
             for (int i = 0; i < s.count; ++i) {
