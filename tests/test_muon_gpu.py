@@ -55,6 +55,36 @@ def test_orthogonalize(dev, rows, cols, out):
         assert torch.equal(got, orthogonalize(g.to(dev), out_dtype=out))
 
 
+@pytest.mark.parametrize("g_dtype,out", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16),
+                                         (torch.float16, torch.bfloat16), (torch.bfloat16, torch.float16)])
+@pytest.mark.parametrize("rows,cols,count", [(129, 15601, 1), (513, 4097, 1), (4097, 513, 1), (1000, 1003, 2), (1470, 1470, 1),
+                                             (200, 1100, 9)])
+def test_16_bit_gradients(dev, rows, cols, count, g_dtype, out):
+    """Large enough that X is held in fp16 alone: what 16-bit numbers hold, fp16 holds times a power of two, but for
+    numbers below 2^-14 of the scaled matrix (mean square about 1), which are off by 2^-25 at most: less than 22 bits."""
+    gen = torch.Generator().manual_seed(rows + cols)
+    for kind, power in (("noise", 0), ("strong", 0), ("noise", -20), ("spikes", 10 if g_dtype == torch.bfloat16 else 0)):
+        g = torch.stack([gradient(rows, cols, "strong" if kind == "strong" else "noise", gen) for _ in range(count)])
+        if kind == "spikes":
+            g *= 1e-3
+            g[:, 3, 5] = 300.0
+            g[:, rows - 1, cols - 1] = -40.0
+        if power:
+            g = g * 2.0 ** power
+        g = g.to(g_dtype)
+        got = orthogonalize(g.to(dev), out_dtype=out)
+        for i in range(0, count, 8):
+            assert off(got[i], polar(g[i])) <= FAR[out], (kind, i)
+        wide = torch.full((count, rows + 2, cols + 3), 7.0, dtype=g_dtype, device=dev)
+        wide[:, 1:-1, 1:-2] = g.to(dev)
+        assert torch.equal(orthogonalize(wide[:, 1:-1, 1:-2], out_dtype=out), got)
+    bad = torch.stack([g[0], torch.zeros_like(g[0]), g[0], g[0], g[0]]).to(dev)
+    bad[2, rows - 1, 3] = float("nan")
+    bad[3, 0, cols - 1] = float("-inf")
+    got = orthogonalize(bad, out_dtype=out)
+    assert torch.equal(got[4], got[0]) and not got[1].any() and torch.isnan(got[2:4]).all()
+
+
 @pytest.mark.parametrize("steps", [1, 2, 3, 4, 6, 7, 9])
 @pytest.mark.parametrize("rows,cols", [(40, 100), (100, 40), (130, 260)])
 def test_any_number_of_steps(dev, rows, cols, steps):
@@ -126,6 +156,20 @@ def test_large_matrix(dev):
     want = polar(torch.eye(rows) * 3.0)[0, 0].item()
     hit = got[at, cols - 1 - 31 * at].float()
     assert ((hit - want).abs() <= want * FAR[torch.bfloat16]).all()
+    got[at, cols - 1 - 31 * at] = 0
+    assert not got.any()
+
+
+def test_large_16_bit_matrix(dev):
+    """The same where X is held in fp16 alone (offsets past 2^32 bytes)."""
+    rows, cols = 130, 1 << 24
+    g = torch.zeros(rows, cols, dtype=torch.float16, device=dev)
+    at = torch.arange(rows, device=dev)
+    g[at, cols - 1 - 31 * at] = 3.0
+    got = orthogonalize(g)
+    want = polar(torch.eye(rows) * 3.0)[0, 0].item()
+    hit = got[at, cols - 1 - 31 * at].float()
+    assert ((hit - want).abs() <= want * FAR[got.dtype]).all()
     got[at, cols - 1 - 31 * at] = 0
     assert not got.any()
 

@@ -25,11 +25,18 @@
 // X is held as a matrix of Frobenius norm `scale` and the factor |G| / (|G| + eps) / scale beside it, a number of its own for
 // each matrix: a gradient far below eps keeps its bits.
 //
+// Where G and the result have 16-bit numbers, X needs no lo ("half": rows of fp16 numbers, zeros up to a multiple of 64): it
+// is G times a power of two, held as fp16 without a rounding (numbers 2^14 below the mean are off by 2^-25 of the mean at
+// most, as in hi + lo), and the factor takes the rest.  X X' is one product instead of three, S X two (S as the planes hi
+// and lo of a row, X' read twice), and X is half the bytes: 4096 x 50,176 9.5 -> 7.2 ms.
+//
 // A matrix of this file, "split": rows of 128-byte blocks, 32 numbers each, 64 bytes of hi and 64 bytes of lo, times
 // a power of two that keeps lo out of the subnormal range; zeros fill a row's last block.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "linear_i8_kernels.hpp"
 #include "tile_product.hpp"
@@ -53,6 +60,7 @@ struct NsShape {
     long long rows, cols;    // of G
     long long l, n;          // short and long side
     long long lk, nk;        // padded to whole blocks of 32
+    long long lh, nh;        // padded to whole blocks of 64 ("half")
     int tall;                // rows > cols: X is G'
     int count;
 };
@@ -183,11 +191,23 @@ __device__ __forceinline__ void split_get_n(const char* p, float (&v)[N]) {
     }
 }
 
-// ---------------------------------------------------------------- G -> X and X', split
+template <int N>
+__device__ __forceinline__ void half_get_n(const char* p, float (&v)[N]) {
+    if constexpr (N == 1) {
+        v[0] = (float)*(const _Float16*)p;
+    } else {
+        typedef _Float16 H __attribute__((ext_vector_type(N)));
+        const H h = *(const H*)p;
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = (float)h[e];
+    }
+}
+
+// ---------------------------------------------------------------- G -> X and X', split or half
 // 64 x 64 numbers of G per workgroup; `nat` gets G's own rows, `tra` its columns, both times scale / |G|.  vec: rows
 // of G (and of the momentum) on 16 bytes and of a multiple of eight numbers.  4096 x 50,176 bf16: 518 us for 2.06 GB
 // (4.0 TB/s).
-template <int DT, bool LIST>
+template <int DT, bool LIST, bool HALF>
 __global__ __launch_bounds__(256) void ns_convert_kernel(NsSource src, NsShape sh, const double* __restrict__ parts, int nparts,
                                                          double eps, double scale, char* __restrict__ nat, long long nat_mat,
                                                          char* __restrict__ tra, long long tra_mat, float* __restrict__ factor, int vec) {
@@ -198,7 +218,11 @@ __global__ __launch_bounds__(256) void ns_convert_kernel(NsSource src, NsShape s
     const T* g = LIST ? (const T*)src.g[mat] : (const T*)src.base + mat * src.stride_b;
     const float* buf = LIST ? src.buf[mat] : nullptr;
     const long long stride = LIST ? sh.cols : src.stride_r;
-    const long long ncp = (sh.cols + 31) & ~31ll, nrp = (sh.rows + 31) & ~31ll;
+    constexpr long long PAD = HALF ? 63 : 31;
+    const long long ncp = (sh.cols + PAD) & ~PAD, nrp = (sh.rows + PAD) & ~PAD;
+    auto place = [](long long row, long long padded, long long col) {
+        return HALF ? row * padded * 2 + col * 2 : split_at(row, padded * 4, col);
+    };
     const unsigned across = (unsigned)((sh.cols + 63) / 64);
     const long long r0 = (long long)(blockIdx.x / across) * 64, c0 = (long long)(blockIdx.x % across) * 64;
     const int line = t >> 2, at = (t & 3) * 16;      // 16 numbers of a line of the tile
@@ -238,8 +262,15 @@ __global__ __launch_bounds__(256) void ns_convert_kernel(NsSource src, NsShape s
     double some = 0.0;
     for (int i = t; i < nparts; i += 256) some += parts[(long long)mat * nparts + i];
     const double sq = block_sum(some, part);
-    const double norm = sqrt(sq), inv = norm == 0.0 ? 0.0 : scale / norm;
-    if (blockIdx.x == 0 && t == 0) factor[mat] = norm == 0.0 ? 0.0f : (float)(norm / (norm + eps) / scale);
+    const double norm = sqrt(sq);
+    double inv = norm == 0.0 ? 0.0 : scale / norm, left = norm / (norm + eps) / scale;
+    if (HALF && norm > 0.0 && norm < 1e300) {
+        int e;
+        frexp(inv, &e);
+        inv = ldexp(1.0, e - 1);                 // the power of two at or below
+        left = 1.0 / ((norm + eps) * inv);
+    }
+    if (blockIdx.x == 0 && t == 0) factor[mat] = norm == 0.0 ? 0.0f : (float)left;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
         if (LIST) v[e] = src.nesterov ? v[e] + src.momentum * m[e] : m[e];
@@ -247,6 +278,17 @@ __global__ __launch_bounds__(256) void ns_convert_kernel(NsSource src, NsShape s
         tile[line][at + e] = v[e];
     }
     auto put = [&](char* p, const float (&x)[16]) {
+        if constexpr (HALF) {
+            v8h a, b;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                a[e] = (_Float16)x[e];
+                b[e] = (_Float16)x[8 + e];
+            }
+            *(v8h*)p = a;
+            *(v8h*)(p + 16) = b;
+            return;
+        }
         float a[8], b[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -256,12 +298,12 @@ __global__ __launch_bounds__(256) void ns_convert_kernel(NsSource src, NsShape s
         split8_put(p, a);
         split8_put(p + 16, b);
     };
-    if (row_in && c0 + at < ncp) put(nat + mat * nat_mat + split_at(r0 + line, ncp * 4, c0 + at), v);
+    if (row_in && c0 + at < ncp) put(nat + mat * nat_mat + place(r0 + line, ncp, c0 + at), v);
     __syncthreads();
     if (c0 + line < sh.cols && r0 + at < nrp) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] = tile[at + e][line];
-        put(tra + mat * tra_mat + split_at(c0 + line, nrp * 4, r0 + at), v);
+        put(tra + mat * tra_mat + place(c0 + line, nrp, r0 + at), v);
     }
 }
 
@@ -275,7 +317,7 @@ struct NsProduct {
     long long ldp;                  // bytes from row to row of P and Q; lk * 4 in E1, E2 and out
     const float* factor;            // of each matrix, or null: k0 times its square
     float k0, k1, k2;
-    int blocks;                     // of 32 numbers along the contraction
+    int blocks;                     // of 128 bytes along the contraction
 };
 struct NsProducts {
     NsProduct job[2];
@@ -351,9 +393,9 @@ __device__ __forceinline__ void ns_store_sym(const NsProduct& p, const NsProduct
     }
 }
 
-template <int BM, int WM, int WN, int STAGES>
+template <class Math, int BM, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(64 * WM * WN, 2) void ns_product_kernel(NsProducts a) {
-    typedef TileProduct<MathSplit, BM, BM, WM, WN, STAGES, true> T;
+    typedef TileProduct<Math, BM, BM, WM, WN, STAGES, true> T;
     YH_TILE_RING(T)
     const NsProduct p = a.job[blockIdx.y];
     const long long per = (long long)a.tiles * a.count;
@@ -590,6 +632,26 @@ __global__ __launch_bounds__((ChainGrid<SIDE, T>::THREADS)) void ns_chain_kernel
     }
 }
 
+// S split -> the planes hi and lo of each row, lh numbers each
+static __global__ __launch_bounds__(256) void ns_planes_kernel(const char* __restrict__ S, long long s_mat, char* __restrict__ planes,
+                                                               long long planes_mat, NsShape sh) {
+    const long long eights = sh.lh / 8, total = sh.l * eights;
+    const char* from = S + blockIdx.y * s_mat;
+    char* to = planes + blockIdx.y * planes_mat;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const long long row = i / eights, col = (i - row * eights) * 8;
+        v4i hi = {0, 0, 0, 0}, lo = hi;
+        if (col < sh.lk) {
+            const char* p = from + split_at(row, sh.lk * 4, col);
+            hi = *(const v4i*)p;
+            lo = *(const v4i*)(p + 64);
+        }
+        char* q = to + row * sh.lh * 4 + col * 2;
+        *(v4i*)q = hi;
+        *(v4i*)(q + sh.lh * 2) = lo;
+    }
+}
+
 // ---------------------------------------------------------------- Y = q X + S X
 enum { NS_OUT_RESULT = 0, NS_OUT_WEIGHT = 1, NS_OUT_SPLIT = 2 };
 
@@ -610,10 +672,11 @@ struct NsApply {
     char *Yn, *Yt;
 };
 
-template <int DT, int OUT, bool TALL, int BM, int BN, int WM, int WN, int STAGES>
+template <int DT, int OUT, bool TALL, bool HALF, int BM, int BN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(64 * WM * WN, 2) void ns_apply_kernel(NsApply a) {
     // a lane's four numbers lie along a row of the result: along n, or along l when X is G'
-    typedef TileProduct<MathSplit, BM, BN, WM, WN, STAGES, !TALL> T;
+    typedef typename std::conditional<HALF, MathHalf, MathSplit>::type Math;
+    typedef TileProduct<Math, BM, BN, WM, WN, STAGES, !TALL> T;
     typedef typename Elem<DT>::T E;
     YH_TILE_RING(T)
     const NsShape& sh = a.sh;
@@ -623,10 +686,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_apply_kernel(NsApply a) {
     const long long mat = id / per, tile = id - mat * per;
     const long long ti = tile % tl, tj = tile / tl;
     typename T::Acc acc[T::TM][T::TN] = {};
-    const long long ld = sh.lk * 4, ldn = sh.nk * 4;
-    const TileOperand A = {a.S + mat * a.s_mat, ld, sh.l, ti * BM, ld - 16};
-    const TileOperand B = {a.Xt + mat * a.xt_mat, ld, sh.n, tj * BN, ld - 16};
-    T::run(A, B, 0, (int)(sh.lk / 32), ring, acc);
+    const long long ld = HALF ? sh.lh * 2 : sh.lk * 4, ldn = HALF ? sh.nh * 2 : sh.nk * 4;
+    const long long lds = HALF ? sh.lh * 4 : ld;         // S: both planes of a row
+    const TileOperand A = {a.S + mat * a.s_mat, lds, sh.l, ti * BM, lds - 16};
+    const TileOperand B = {a.Xt + mat * a.xt_mat, ld, sh.n, tj * BN, ld - 16, HALF ? (int)(sh.lh / 64) : 1 << 30};
+    T::run(A, B, 0, (int)(lds / TILE_BLOCK_BYTES), ring, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const char* x = TALL ? a.Xt + mat * a.xt_mat : a.X + mat * a.x_mat;
     const long long ldx = TALL ? ld : ldn;
@@ -652,7 +716,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_apply_kernel(NsApply a) {
             constexpr int W = (int)(sizeof(v) / sizeof(float));
             if (row >= rows || col >= cols_pad) return false;
             float e[W];
-            split_get_n<W>(x + split_at(row, ldx, col), e);
+            if constexpr (HALF) half_get_n<W>(x + row * ldx + col * 2, e);
+            else split_get_n<W>(x + split_at(row, ldx, col), e);
 #pragma unroll
             for (int k = 0; k < W; ++k) v[k] += k1 * e[k];
             return true;

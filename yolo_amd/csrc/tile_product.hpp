@@ -1,12 +1,13 @@
 // Tile products on the matrix cores (gfx950): D = A * B' for two operands whose rows lie along the
-// contraction, 128 bytes of a row at a time.  Two arithmetics share the data path, since a lane's
-// share of a fragment is 16 bytes in both:
+// contraction, 128 bytes of a row at a time.  Three arithmetics share the data path, since a lane's
+// share of a fragment is 16 bytes in all:
 //
 //   MathI8     a 128-byte block of a row is 128 signed bytes; two 16x16x64 products per 16x16
 //              piece of D, exact in int32.
 //   MathSplit  a block is 32 numbers in two halves: 64 bytes of their leading parts (fp16), then 64
 //              bytes of what fp16 leaves over (fp16 again): x = hi + lo to 22 bits.  Three 16x16x32
 //              products, hi*hi + hi*lo + lo*hi, in fp32; lo*lo is below 2^-22 of the product.
+//   MathHalf   a block is 64 fp16 numbers; two 16x16x32 products.
 //
 // Lane l of a wavefront holds, of a 16-row fragment, row l % 16 and the bytes 16 * (l / 16) .. + 15 of a
 // 64-byte half; D's piece has row (first operand) 4 * (l / 16) + r in register r and column (second
@@ -43,6 +44,15 @@ struct MathSplit {
     }
 };
 
+// a block is 64 fp16 numbers, for matrices that fp16 holds exactly
+struct MathHalf {
+    using Acc = v4f;
+    static constexpr int PASSES = 2;
+    template <int PASS> static __device__ __forceinline__ void mma(Acc& d, const v4i (&p)[2], const v4i (&q)[2]) {
+        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, p[PASS]), __builtin_bit_cast(v8h, q[PASS]), d, 0, 0, 0);
+    }
+};
+
 // acc[j] += fragment a * fragment b[j] (or the other way round), pass by pass: consecutive instructions write
 // different registers
 template <class Math, bool ROWS_B, int PASS, int TN>
@@ -69,6 +79,7 @@ struct TileOperand {
     long long rows;
     long long first;
     long long last_chunk;   // below 2^31
+    int turn = 1 << 30;     // blocks of a row: from there on they are read again from the first
 };
 
 // A workgroup of WM x WN wavefronts computes BM x BN numbers over the blocks [kb0, kb1) of the contraction.
@@ -140,7 +151,8 @@ struct TileProduct {
         };
         auto load = [&](LdsPtr s, int kb) {
             const int off = kb * TILE_BLOCK_BYTES + chunk;
-            const int oa = off < last_a ? off : last_a, ob = off < last_b ? off : last_b;
+            const int offb = (kb < B.turn ? kb : kb - B.turn) * TILE_BLOCK_BYTES + chunk;
+            const int oa = off < last_a ? off : last_a, ob = offb < last_b ? offb : last_b;
 #pragma unroll
             for (int i = 0; i < LA; ++i) to_lds(pa[i] + oa, s + (group + i * 8 * WAVES) * TILE_BLOCK_BYTES);
 #pragma unroll

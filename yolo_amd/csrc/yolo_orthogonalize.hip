@@ -57,6 +57,8 @@ NsShape shape_of(int64_t rows, int64_t cols, int count) {
     s.n = s.tall ? rows : cols;
     s.lk = (s.l + 31) & ~31ll;
     s.nk = (s.n + 31) & ~31ll;
+    s.lh = (s.l + 63) & ~63ll;
+    s.nh = (s.n + 63) & ~63ll;
     s.count = count;
     return s;
 }
@@ -72,9 +74,10 @@ int check_sizes(int64_t count, int64_t rows, int64_t cols) {
 }
 
 struct Layout {
-    size_t parts, factor, x, xt, xt2, a, r0, r1, t, s0, s1, partial, total;
+    size_t parts, factor, x, xt, xt2, a, r0, r1, t, s0, s1, partial, total;      // the planes of S go where xt2 would be
     long long x_mat, xt_mat, sq_mat;
     int norm_blocks;
+    bool half;
     int gram, tiles, slices, per_slice;      // X X': kind of tile, tiles on and below the diagonal, slices
     int square, square_tiles;                // the l x l products
 };
@@ -84,15 +87,17 @@ inline int triangle_tiles(int64_t l, int b) {
     return (int)(side * (side + 1) / 2);
 }
 
-Layout layout_for(const NsShape& s) {
+// half: X in fp16 alone
+Layout layout_for(const NsShape& s, bool half) {
     Layout w = {};
+    w.half = half;
     int64_t nb = (s.rows * s.cols + 4095) / 4096;
     w.norm_blocks = (int)(nb < 1 ? 1 : nb > NS_NORM_BLOCKS ? NS_NORM_BLOCKS : nb);
-    w.x_mat = s.l * s.nk * 4;
-    w.xt_mat = s.n * s.lk * 4;
+    w.x_mat = half ? s.l * s.nh * 2 : s.l * s.nk * 4;
+    w.xt_mat = half ? s.n * s.lh * 2 : s.n * s.lk * 4;
     w.sq_mat = s.l * s.lk * 4;
     // the contraction of X X' is cut when the tiles alone do not fill the card
-    const int64_t blocks = s.nk / 32;
+    const int64_t blocks = half ? s.nh / 64 : s.nk / 32;
     double best = 0.0, best_square = 0.0;
     for (int k = 0; k < TILE_KINDS; ++k) {
         const int t = triangle_tiles(s.l, kTiles[k].bm);
@@ -123,7 +128,7 @@ Layout layout_for(const NsShape& s) {
     w.factor = take((size_t)s.count * 4);
     w.x = take((size_t)s.count * w.x_mat);
     w.xt = take((size_t)s.count * w.xt_mat);
-    w.xt2 = take((size_t)s.count * w.xt_mat);
+    w.xt2 = take((size_t)s.count * (half ? s.l * s.lh * 4 : w.xt_mat));
     w.a = take((size_t)s.count * w.sq_mat);
     w.r0 = take((size_t)s.count * w.sq_mat);
     w.r1 = take((size_t)s.count * w.sq_mat);
@@ -144,13 +149,13 @@ struct Sink {
     float decay, step;
 };
 
-template <int DT, int OUT, bool TALL, int BM, int BN, int WM, int WN, int STAGES>
+template <int DT, int OUT, bool TALL, bool HALF, int BM, int BN, int WM, int WN, int STAGES>
 void apply_tiles(const NsApply& a, hipStream_t st) {
     const int64_t tiles = ((a.sh.l + BM - 1) / BM) * ((a.sh.n + BN - 1) / BN) * a.sh.count;
-    hipLaunchKernelGGL((ns_apply_kernel<DT, OUT, TALL, BM, BN, WM, WN, STAGES>), dim3((unsigned)tiles), dim3(64 * WM * WN), 0, st, a);
+    hipLaunchKernelGGL((ns_apply_kernel<DT, OUT, TALL, HALF, BM, BN, WM, WN, STAGES>), dim3((unsigned)tiles), dim3(64 * WM * WN), 0, st, a);
 }
 
-template <int DT, int OUT, bool TALL>
+template <int DT, int OUT, bool TALL, bool HALF = false>
 int apply(const NsApply& a, hipStream_t st) {
     int kind = 0;
     double best = 0.0;
@@ -163,10 +168,10 @@ int apply(const NsApply& a, hipStream_t st) {
             kind = k;
         }
     }
-    if (kind == TILE_LARGE) apply_tiles<DT, OUT, TALL, 128, 256, 2, 4, 3>(a, st);
-    else if (kind == TILE_128) apply_tiles<DT, OUT, TALL, 128, 128, 2, 4, 4>(a, st);
-    else if (kind == TILE_64) apply_tiles<DT, OUT, TALL, 64, 64, 2, 2, 4>(a, st);
-    else apply_tiles<DT, OUT, TALL, 32, 32, 2, 2, 4>(a, st);
+    if (kind == TILE_LARGE) apply_tiles<DT, OUT, TALL, HALF, 128, 256, 2, 4, 3>(a, st);
+    else if (kind == TILE_128) apply_tiles<DT, OUT, TALL, HALF, 128, 128, 2, 4, 4>(a, st);
+    else if (kind == TILE_64) apply_tiles<DT, OUT, TALL, HALF, 64, 64, 2, 2, 4>(a, st);
+    else apply_tiles<DT, OUT, TALL, HALF, 32, 32, 2, 2, 4>(a, st);
     return launch_status();
 }
 
@@ -177,22 +182,31 @@ int apply_as(int dt, bool tall, const NsApply& a, hipStream_t st) {
     return tall ? apply<DT_BF16, OUT, true>(a, st) : apply<DT_BF16, OUT, false>(a, st);
 }
 
-template <int BM, int WM, int WN, int STAGES>
+// X in fp16 alone serves 16-bit results
+int apply_half(int dt, bool tall, const NsApply& a, hipStream_t st) {
+    if (dt == YH_F16) return tall ? apply<DT_F16, NS_OUT_RESULT, true, true>(a, st) : apply<DT_F16, NS_OUT_RESULT, false, true>(a, st);
+    return tall ? apply<DT_BF16, NS_OUT_RESULT, true, true>(a, st) : apply<DT_BF16, NS_OUT_RESULT, false, true>(a, st);
+}
+
+template <class Math, int BM, int WM, int WN, int STAGES>
 int products_of(const NsProducts& a, int jobs, hipStream_t st) {
     const unsigned grid = (unsigned)((int64_t)a.tiles * a.count * a.slices);
-    hipLaunchKernelGGL((ns_product_kernel<BM, WM, WN, STAGES>), dim3(grid, (unsigned)jobs), dim3(64 * WM * WN), 0, st, a);
+    hipLaunchKernelGGL((ns_product_kernel<Math, BM, WM, WN, STAGES>), dim3(grid, (unsigned)jobs), dim3(64 * WM * WN), 0, st, a);
     if (const int rc = launch_status()) return rc;
     if (a.slices > 1)
         hipLaunchKernelGGL((ns_join_kernel<BM, WM, WN, STAGES>), dim3((unsigned)(a.tiles * a.count)), dim3(64 * WM * WN), 0, st, a);
     return launch_status();
 }
 
-int products(int kind, const NsProducts& a, int jobs, hipStream_t st) {
-    if (kind == TILE_LARGE) return products_of<192, 2, 4, 3>(a, jobs, st);
-    if (kind == TILE_128) return products_of<128, 2, 4, 4>(a, jobs, st);
-    if (kind == TILE_64) return products_of<64, 2, 2, 4>(a, jobs, st);
-    return products_of<32, 2, 2, 4>(a, jobs, st);
+template <class Math>
+int products_in(int kind, const NsProducts& a, int jobs, hipStream_t st) {
+    if (kind == TILE_LARGE) return products_of<Math, 192, 2, 4, 3>(a, jobs, st);
+    if (kind == TILE_128) return products_of<Math, 128, 2, 4, 4>(a, jobs, st);
+    if (kind == TILE_64) return products_of<Math, 64, 2, 2, 4>(a, jobs, st);
+    return products_of<Math, 32, 2, 2, 4>(a, jobs, st);
 }
+
+int products(int kind, const NsProducts& a, int jobs, hipStream_t st) { return products_in<MathSplit>(kind, a, jobs, st); }
 
 constexpr int kChainSide = 128;     // A up to this size is worked on by one workgroup
 
@@ -216,10 +230,19 @@ int load(const NsSource& src, const NsShape& s, const Layout& w, char* ws, doubl
     if (const int rc = launch_status()) return rc;
     char* x = ws + w.x;
     char* xt = ws + w.xt;
-    hipLaunchKernelGGL((ns_convert_kernel<DT, LIST>),
-                       dim3((unsigned)(((s.cols + 63) / 64) * ((s.rows + 63) / 64)), (unsigned)s.count), dim3(256), 0, st,
-                       src, s, (const double*)(ws + w.parts), w.norm_blocks, eps, scale, s.tall ? xt : x,
-                       s.tall ? w.xt_mat : w.x_mat, s.tall ? x : xt, s.tall ? w.x_mat : w.xt_mat, (float*)(ws + w.factor), vec);
+    const dim3 grid((unsigned)(((s.cols + 63) / 64) * ((s.rows + 63) / 64)), (unsigned)s.count);
+    auto convert = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, src, s, (const double*)(ws + w.parts), w.norm_blocks, eps, scale,
+                           s.tall ? xt : x, s.tall ? w.xt_mat : w.x_mat, s.tall ? x : xt, s.tall ? w.x_mat : w.xt_mat,
+                           (float*)(ws + w.factor), vec);
+    };
+    if constexpr (!LIST && DT != DT_F32) {
+        if (w.half) {
+            convert(ns_convert_kernel<DT, LIST, true>);
+            return launch_status();
+        }
+    }
+    convert(ns_convert_kernel<DT, LIST, false>);
     return launch_status();
 }
 
@@ -230,6 +253,22 @@ int load_as(int dt, const NsSource& src, const NsShape& s, const Layout& w, char
     return load<DT_BF16, LIST>(src, s, w, ws, eps, scale, st);
 }
 
+// how many of `left` steps one X X' serves: while a^steps stays below 64 (fp32 results) or 512
+int group_steps(float a, int left, int out_dtype) {
+    const double by = fabs((double)a), limit = out_dtype == YH_F32 ? 64.0 : 512.0;
+    int len = 1;
+    for (double grown = by * by; len < left && grown <= limit; grown *= by) ++len;
+    return len;
+}
+
+// X in fp16 alone: 16-bit numbers, all steps on one X X', and enough of them to pay for the launch that lays S out in
+// planes (a call in us, split / half: 192x576 85.6 / 90.1, 512x512 113 / 117, 256x4096 104.5 / 102.3, 512x2304 129 / 127,
+// 4x512x2304 202 / 195, 1470x4096 475 / 443, 4x1024x9216 897 / 740, 4096x50,176 9520 / 7210)
+bool half_for(const NsShape& s, int g_dtype, int out_dtype, float a, int steps) {
+    return g_dtype != YH_F32 && out_dtype != YH_F32 && s.l > 128 && (double)s.l * (double)s.n * s.count >= 1e6 &&
+           group_steps(a, steps, out_dtype) == steps;
+}
+
 // G is in the workspace as X and X' (of norm `scale`, their factor beside them); the steps, and the result to `sink`
 int run_steps(const NsShape& s, const Layout& w, char* ws, double scale, float a, float b, float c, int steps, const Sink& sink,
               hipStream_t st) {
@@ -238,7 +277,6 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, double scale, float a
     const int lb = (int)(s.lk / 32);
     const float* factor = (const float*)(ws + w.factor);
     double rest = 1.0, held = scale;           // X_j = rest * factor * (what is held), which has grown from norm `held`
-    const double limit = sink.dtype == YH_F32 ? 64.0 : 512.0;
     NsProducts base = {};
     base.l = s.l;
     base.lk = s.lk;
@@ -263,8 +301,7 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, double scale, float a
     };
     int done = 0;
     while (done < steps) {
-        int len = 1;
-        for (double grown = fabs((double)a) * fabs((double)a); done + len < steps && grown <= limit; grown *= fabs((double)a)) ++len;
+        const int len = group_steps(a, steps - done, sink.dtype);
         // A = X X'
         NsProducts gram = base;
         gram.tiles = w.tiles;
@@ -274,9 +311,9 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, double scale, float a
         gram.job[0] = job(X, X, A, (float)(kScaleA * rest * rest), nullptr, 0.0f, nullptr, 0.0f);
         gram.job[0].factor = factor;
         gram.job[0].p_mat = w.x_mat;
-        gram.job[0].ldp = s.nk * 4;
-        gram.job[0].blocks = (int)(s.nk / 32);
-        if (const int rc = products(w.gram, gram, 1, st)) return rc;
+        gram.job[0].ldp = w.half ? s.nh * 2 : s.nk * 4;
+        gram.job[0].blocks = (int)(gram.job[0].ldp / TILE_BLOCK_BYTES);
+        if (const int rc = w.half ? products_in<MathHalf>(w.gram, gram, 1, st) : products(w.gram, gram, 1, st)) return rc;
         double q = a;                          // Q = q + S
         const char* Q = nullptr;
         float sq = 0.0f;
@@ -367,7 +404,14 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, double scale, float a
             if (aligned(sink.out, 16) && (sink.out_r * e) % 16 == 0 && (sink.out_b * e) % 16 == 0) ap.store = STORE_16;
             else if (aligned(sink.out, 2 * e) && sink.out_r % 2 == 0 && sink.out_b % 2 == 0) ap.store = STORE_PAIR;
             else ap.store = STORE_ONE;
-            if (const int rc = apply_as<NS_OUT_RESULT>(sink.dtype, s.tall, ap, st)) return rc;
+            if (w.half) {
+                hipLaunchKernelGGL(ns_planes_kernel, dim3((unsigned)((s.l * s.lh / 8 + 1023) / 1024), (unsigned)s.count), dim3(256), 0, st, Q,
+                                   w.sq_mat, Xt_next, (long long)(s.l * s.lh * 4), s);
+                if (const int rc = launch_status()) return rc;
+                ap.S = Xt_next;
+                ap.s_mat = s.l * s.lh * 4;
+                if (const int rc = apply_half(sink.dtype, s.tall, ap, st)) return rc;
+            } else if (const int rc = apply_as<NS_OUT_RESULT>(sink.dtype, s.tall, ap, st)) return rc;
         }
     }
     return YH_OK;
@@ -388,7 +432,9 @@ extern "C" {
 
 size_t yh_orthogonalize_workspace_bytes(int64_t count, int64_t rows, int64_t cols) {
     if (check_sizes(count, rows, cols) != YH_OK || count == 0) return 0;
-    return layout_for(shape_of(rows, cols, (int)count)).total;
+    const NsShape s = shape_of(rows, cols, (int)count);
+    const size_t split = layout_for(s, false).total, half = layout_for(s, true).total;
+    return split > half ? split : half;
 }
 
 int yh_orthogonalize(const void* g, int g_dtype, int64_t g_stride, int64_t ldg, void* out, int out_dtype, int64_t out_stride,
@@ -402,8 +448,8 @@ int yh_orthogonalize(const void* g, int g_dtype, int64_t g_stride, int64_t ldg, 
     if (count == 0) return YH_OK;
     if (!g || !out) return YH_ERR_NULL;
     const NsShape s = shape_of(rows, cols, (int)count);
-    const Layout w = layout_for(s);
-    if (!workspace || workspace_bytes < w.total) return YH_ERR_WORKSPACE;
+    const Layout w = layout_for(s, half_for(s, g_dtype, out_dtype, a, steps));
+    if (!workspace || workspace_bytes < yh_orthogonalize_workspace_bytes(count, rows, cols)) return YH_ERR_WORKSPACE;
     if (!aligned(g, dtype_bytes(g_dtype)) || !aligned(out, dtype_bytes(out_dtype)) || !aligned(workspace, 256)) return YH_ERR_ALIGN;
     hipStream_t st = (hipStream_t)stream;
     char* ws = (char*)workspace;
@@ -441,8 +487,8 @@ int yh_muon_step(void* const* params, int p_dtype, const void* const* grads, int
         src.buf[i] = momenta[i];
     }
     const NsShape s = shape_of(rows, cols, count);
-    const Layout w = layout_for(s);
-    if (!workspace || workspace_bytes < w.total) return YH_ERR_WORKSPACE;
+    const Layout w = layout_for(s, false);
+    if (!workspace || workspace_bytes < yh_orthogonalize_workspace_bytes(count, rows, cols)) return YH_ERR_WORKSPACE;
     if (!aligned(workspace, 256)) return YH_ERR_ALIGN;
     src.momentum = momentum;
     src.nesterov = nesterov != 0;
