@@ -146,6 +146,52 @@ def test_scale_zeros_and_what_is_not_a_number(dev):
     assert off(orthogonalize(spike, out_dtype=torch.float32), polar(spike.cpu())) <= 1e-4
 
 
+def test_many_steps_of_tiny_gradients(dev):
+    """|X_0| far below 1 and enough steps for it to grow back: what is held of X grows by 3.4445 a step until the singular
+    values have reached their range, and stays inside fp16's."""
+    gen = torch.Generator().manual_seed(6)
+    line = torch.zeros(40, 90)
+    line[7, 30] = 1.0                                     # all of the norm in one number
+    noise = torch.randn(40, 90, generator=gen)
+    noise /= noise.norm()
+    wide = torch.randn(200, 260, generator=gen)
+    for name, g in (("line", line), ("noise", noise), ("wide", wide / wide.norm()), ("tall", (wide / wide.norm()).t().contiguous())):
+        for norm, steps in ((1e-11, 9), (1e-12, 12), (1e-13, 16), (1e-15, 20), (1e-25, 40), (1.0, 30)):
+            small = g * norm
+            for out in (torch.float32, torch.float16):
+                got, want = orthogonalize(small.to(dev), steps=steps, out_dtype=out), polar(small, steps)
+                assert torch.isfinite(got).all() and got.any(), (name, norm, steps)
+                if want.norm() > 1e-3 and name == "line":
+                    assert off(got, want) <= FAR[out], (name, norm, steps)
+
+
+@pytest.mark.parametrize("coeffs,steps", [((2.0, 2.0, 1.0), 1), ((100.0, -99.0, 0.0), 1), ((1.0, 60.0, -59.0), 1), ((0.5, 0.0, 0.0), 40),
+                                          ((0.0, 1.0, 0.0), 1), ((-1.5, 0.5, 0.0), 7), ((1.5, -0.5, 0.0), 64)])
+def test_coefficients_within_range(dev, coeffs, steps):
+    gen = torch.Generator().manual_seed(8)
+    for rows, cols in ((30, 70), (150, 140)):
+        g = gradient(rows, cols, "noise", gen)
+        got = orthogonalize(g.to(dev), steps=steps, coeffs=coeffs, out_dtype=torch.float32)
+        assert off(got, polar(g, steps, coeffs)) <= 1e-4
+
+
+def test_state_dict_of_16_bit_weights(dev):
+    torch.manual_seed(1)
+    w = torch.nn.Parameter(torch.randn(24, 40, device=dev, dtype=torch.bfloat16))
+    optim = Muon([w], lr=0.1)
+    grads = [torch.randn_like(w) for _ in range(3)]
+    for g in grads[:2]:
+        w.grad = g
+        optim.step()
+    other = torch.nn.Parameter(w.detach().clone())
+    loaded = Muon([other])
+    loaded.load_state_dict(optim.state_dict())
+    w.grad, other.grad = grads[2], grads[2].clone()
+    optim.step()
+    loaded.step()
+    assert torch.equal(w.detach(), other.detach())
+
+
 def test_large_matrix(dev):
     """Offsets past 2^32 bytes in the split copies (70 x 2^24 numbers of 4 bytes)."""
     rows, cols = 70, 1 << 24

@@ -130,3 +130,37 @@ def test_python_layer_refuses():
     assert layer.weight.shape == (3, 64) and layer.weight.stride(0) == 128
     with pytest.raises(ValueError, match="output channels"):
         YOLOv1Head().postprocess_linear(x, layer)
+
+
+@pytest.mark.parametrize("coeffs,steps", [((3.0, -4.0, 2.0), 5), ((2.0, 2.0, 1.0), 2), ((121.0, 0.0, 0.0), 1), ((1e30, 0.0, 0.0), 1),
+                                          ((0.0, 500.0, -500.0), 1), ((1.0, 121.0, 0.0), 1), ((100.0, -99.0, 0.0), 2),
+                                          ((3e38, 3e38, 3e38), 64)])
+def test_coefficients_that_leave_the_range_are_refused(coeffs, steps):
+    """In [0, 1] the singular values of these reach s^2, |b s^2 + c s^4| or s^2 |a + b s^2 + c s^4| past 120 before a step;
+    shown here on a grid."""
+    s, worst = torch.linspace(0, 1, 20001, dtype=torch.float64), 0.0
+    a, b, c = coeffs
+    for _ in range(steps):
+        z = s * s
+        r = b * z + c * z * z
+        worst = max(worst, z.max().item(), r.abs().max().item(), (z * (a + r)).abs().max().item())
+        s = (s * (a + r)).clamp(-1e9, 1e9)
+    lib, lists = _lib.load(), (ctypes.c_void_p * 1)(FAKE)
+    assert worst > 120
+    assert lib.yh_orthogonalize(FAKE, _lib.YH_F32, 128, 16, FAKE, _lib.YH_F32, 128, 16, 1, 8, 16, *coeffs, steps, 1e-7, FAKE, BIG,
+                                None) == _lib.YH_ERR_ARG
+    assert lib.yh_muon_step(lists, _lib.YH_F32, lists, _lib.YH_F32, lists, 1, 8, 16, 0.1, 0.9, 1, 0.0, 1.0, *coeffs, steps, 1e-7,
+                            FAKE, BIG, None) == _lib.YH_ERR_ARG
+
+
+def test_momenta_stay_fp32_through_a_state_dict():
+    """torch casts the state of a 16-bit weight to 16 bits when it is loaded; momenta are not."""
+    weights = [torch.nn.Parameter(torch.zeros(3, 5, dtype=torch.bfloat16)), torch.nn.Parameter(torch.zeros(4, 2))]
+    first, second = Muon(weights), Muon(weights, lr=1.0)
+    for p in weights:
+        first.state[p]["momentum_buffer"] = torch.randn(p.shape)
+    second.load_state_dict(first.state_dict())
+    for p in weights:
+        got, saved = (o.state[p]["momentum_buffer"] for o in (second, first))
+        assert got.dtype == torch.float32 and torch.equal(got, saved) and got.data_ptr() != saved.data_ptr()
+    assert second.param_groups[0]["lr"] == 0.02

@@ -404,7 +404,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_i8_tile_kernel(LinearI
     }
 }
 
-// the slices' sums (integers: any order gives the same), scales, bias
 // Up to 16 rows a workgroup (blockIdx.y: which): the weight is read once, straight into registers, and that is what bounds
 // it.  A workgroup of 16 wavefronts takes 16 channels; a wavefront takes every 16th block of 128 bytes of their rows, four
 // blocks (8 KB) on their way while four are worked on; the 16 sums meet in LDS.  STAGE: every workgroup brings the rows of x
@@ -539,6 +538,7 @@ __global__ __launch_bounds__(1024) void linear_i8_rows_kernel(LinearI8Args a, co
     }
 }
 
+// the slices' sums (integers: any order gives the same), scales, bias
 template <int DT>
 __global__ __launch_bounds__(256) void linear_i8_join_kernel(LinearI8Args a) {
     const long long quads = (a.N + 3) / 4, total = a.M * quads, plane = a.M * a.N;

@@ -19,11 +19,12 @@
 // Every matrix is therefore held as two fp16 numbers, hi + lo: 22 bits, three matrix-core products for one, fp32
 // sums.  An error of A grows by a^2 a step, which limits how many steps one A may serve: five end 1e-5 to 2e-4 off,
 // three and two with a fresh A in between 3e-6 to 3e-5, an A for every step 2e-6 to 2e-5 -- the last is what fp32
-// arithmetic gives.  The entry points form a new A when a^steps would pass 64 (fp32 results) or 512 (16-bit
+// arithmetic gives.  The entry points form a new A when a^steps would pass 64 (fp32 results) or 511 (16-bit
 // results, whose own rounding is 2e-3).
 //
 // X is held as a matrix of Frobenius norm `scale` and the factor |G| / (|G| + eps) / scale beside it, a number of its own for
-// each matrix: a gradient far below eps keeps its bits.
+// each matrix: a gradient far below eps keeps its bits.  What is held grows with the steps, by `growth` as long as the singular
+// values are small and until they reach `top`, so each group of steps begins at a scale (and factor) with room for that.
 //
 // Where G and the result have 16-bit numbers, X needs no lo ("half": rows of fp16 numbers, zeros up to a multiple of 64): it
 // is G times a power of two, held as fp16 without a rounding (numbers 2^14 below the mean are off by 2^-25 of the mean at
@@ -42,6 +43,14 @@
 #include "tile_product.hpp"
 
 namespace yh {
+
+constexpr int NS_MAX_GROUPS = 64;
+struct NsHold {
+    int groups;
+    double scale;                    // of the first group
+    // before group g, powers of two: small singular values have grown by less than growth[g], none has reached top[g]
+    short growth[NS_MAX_GROUPS], top[NS_MAX_GROUPS];
+};
 
 constexpr int NS_MAX_LIST = 32;      // matrices of one call that are handed over as a list of pointers
 constexpr int NS_NORM_BLOCKS = 1024; // partial sums of squares of a matrix, at most
@@ -209,8 +218,9 @@ __device__ __forceinline__ void half_get_n(const char* p, float (&v)[N]) {
 // (4.0 TB/s).
 template <int DT, bool LIST, bool HALF>
 __global__ __launch_bounds__(256) void ns_convert_kernel(NsSource src, NsShape sh, const double* __restrict__ parts, int nparts,
-                                                         double eps, double scale, char* __restrict__ nat, long long nat_mat,
-                                                         char* __restrict__ tra, long long tra_mat, float* __restrict__ factor, int vec) {
+                                                         double eps, NsHold hold, char* __restrict__ nat, long long nat_mat,
+                                                         char* __restrict__ tra, long long tra_mat, float* __restrict__ factor,
+                                                         float* __restrict__ hop, int vec) {
     typedef typename Elem<DT>::T T;
     __shared__ float tile[64][65];
     __shared__ double part[4];
@@ -263,14 +273,23 @@ __global__ __launch_bounds__(256) void ns_convert_kernel(NsSource src, NsShape s
     for (int i = t; i < nparts; i += 256) some += parts[(long long)mat * nparts + i];
     const double sq = block_sum(some, part);
     const double norm = sqrt(sq);
-    double inv = norm == 0.0 ? 0.0 : scale / norm, left = norm / (norm + eps) / scale;
+    double inv = norm == 0.0 ? 0.0 : hold.scale / norm;
     if (HALF && norm > 0.0 && norm < 1e300) {
         int e;
         frexp(inv, &e);
         inv = ldexp(1.0, e - 1);                 // the power of two at or below
-        left = 1.0 / ((norm + eps) * inv);
     }
-    if (blockIdx.x == 0 && t == 0) factor[mat] = norm == 0.0 ? 0.0f : (float)left;
+    if (blockIdx.x == 0 && t < hold.groups) {
+        // X_g = factor[g] times what is held; hop[g]: from what is held in group g - 1 to what is held in group g
+        const double unit = norm / (norm + eps);                   // |X_0|
+        auto scale_of = [&](int g) {
+            const int most = hold.top[g] - ilogb(unit);
+            return ldexp(1.0, 15 - (hold.growth[g] < most ? hold.growth[g] : most));
+        };
+        const double now = t == 0 ? inv * norm : scale_of(t), before = t == 1 ? inv * norm : t > 1 ? scale_of(t - 1) : now;
+        factor[t * sh.count + mat] = norm == 0.0 ? 0.0f : (float)(unit / now);
+        hop[t * sh.count + mat] = norm == 0.0 ? 0.0f : (float)(now / before);
+    }
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
         if (LIST) v[e] = src.nesterov ? v[e] + src.momentum * m[e] : m[e];
@@ -659,7 +678,7 @@ struct NsApply {
     const char *S, *X, *Xt;
     long long s_mat, x_mat, xt_mat;
     NsShape sh;
-    const float* factor;             // of each matrix: Y times it, where it leaves (NS_OUT_SPLIT keeps it apart)
+    const float* factor;             // of each matrix: Y times it (NS_OUT_SPLIT: to what is held next)
     float k0, k1;                    // Y = k0 * (S X) + k1 * X
     // NS_OUT_RESULT
     void* out;
@@ -700,7 +719,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_apply_kernel(NsApply a) {
     static_assert((T::WAVES + 1) / 2 * TURN_BYTES<ALONG> <= T::HALF, "fits two stages");
     __syncthreads();
     LdsPtr turn = (wave & 1 ? ring[1] : ring[0]) + (wave >> 1) * TURN_BYTES<ALONG>;
-    const float factor = OUT == NS_OUT_SPLIT ? 1.0f : a.factor[mat];
+    const float factor = a.factor[mat];
     const float k0 = a.k0 * factor, k1 = a.k1 * factor;
 #pragma unroll
     for (int i = 0; i < ACROSS; ++i) {

@@ -45,7 +45,7 @@ double tile_time(const TileKind& k, int64_t wgs, int64_t blocks) {
     return (double)((wgs + at_once - 1) / at_once) * ((double)blocks * (k.block + k.more * (double)(together - 1)) + k.start);
 }
 
-// powers of two the split matrices are held at: A and T up to about 1.5, R up to 127, S up to 1023
+// powers of two the split matrices are held at: A, R and T up to 120, S up to 1022 (steps_in_groups)
 constexpr float kScaleA = 512.0f, kScaleR = 512.0f, kScaleS = 64.0f;
 
 NsShape shape_of(int64_t rows, int64_t cols, int count) {
@@ -74,7 +74,7 @@ int check_sizes(int64_t count, int64_t rows, int64_t cols) {
 }
 
 struct Layout {
-    size_t parts, factor, x, xt, xt2, a, r0, r1, t, s0, s1, partial, total;      // the planes of S go where xt2 would be
+    size_t parts, factor, hop, x, xt, xt2, a, r0, r1, t, s0, s1, partial, total;      // the planes of S go where xt2 would be
     long long x_mat, xt_mat, sq_mat;
     int norm_blocks;
     bool half;
@@ -125,7 +125,8 @@ Layout layout_for(const NsShape& s, bool half) {
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t at = off; off += up256(bytes); return at; };
     w.parts = take((size_t)s.count * w.norm_blocks * 8);
-    w.factor = take((size_t)s.count * 4);
+    w.factor = take((size_t)s.count * NS_MAX_GROUPS * 4);
+    w.hop = take((size_t)s.count * NS_MAX_GROUPS * 4);
     w.x = take((size_t)s.count * w.x_mat);
     w.xt = take((size_t)s.count * w.xt_mat);
     w.xt2 = take((size_t)s.count * (half ? s.l * s.lh * 4 : w.xt_mat));
@@ -220,7 +221,7 @@ int chain(const NsChain& c, int count, hipStream_t st) {
 }
 
 template <int DT, bool LIST>
-int load(const NsSource& src, const NsShape& s, const Layout& w, char* ws, double eps, double scale, hipStream_t st) {
+int load(const NsSource& src, const NsShape& s, const Layout& w, char* ws, double eps, const NsHold& hold, hipStream_t st) {
     bool on16 = LIST || (aligned(src.base, 16) && src.stride_r % 8 == 0 && src.stride_b % 8 == 0);
     if (LIST)
         for (int i = 0; i < s.count; ++i) on16 = on16 && aligned(src.g[i], 16) && aligned(src.buf[i], 16);
@@ -232,9 +233,9 @@ int load(const NsSource& src, const NsShape& s, const Layout& w, char* ws, doubl
     char* xt = ws + w.xt;
     const dim3 grid((unsigned)(((s.cols + 63) / 64) * ((s.rows + 63) / 64)), (unsigned)s.count);
     auto convert = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, src, s, (const double*)(ws + w.parts), w.norm_blocks, eps, scale,
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, src, s, (const double*)(ws + w.parts), w.norm_blocks, eps, hold,
                            s.tall ? xt : x, s.tall ? w.xt_mat : w.x_mat, s.tall ? x : xt, s.tall ? w.x_mat : w.xt_mat,
-                           (float*)(ws + w.factor), vec);
+                           (float*)(ws + w.factor), (float*)(ws + w.hop), vec);
     };
     if constexpr (!LIST && DT != DT_F32) {
         if (w.half) {
@@ -247,36 +248,77 @@ int load(const NsSource& src, const NsShape& s, const Layout& w, char* ws, doubl
 }
 
 template <bool LIST>
-int load_as(int dt, const NsSource& src, const NsShape& s, const Layout& w, char* ws, double eps, double scale, hipStream_t st) {
-    if (dt == YH_F32) return load<DT_F32, LIST>(src, s, w, ws, eps, scale, st);
-    if (dt == YH_F16) return load<DT_F16, LIST>(src, s, w, ws, eps, scale, st);
-    return load<DT_BF16, LIST>(src, s, w, ws, eps, scale, st);
+int load_as(int dt, const NsSource& src, const NsShape& s, const Layout& w, char* ws, double eps, const NsHold& hold, hipStream_t st) {
+    if (dt == YH_F32) return load<DT_F32, LIST>(src, s, w, ws, eps, hold, st);
+    if (dt == YH_F16) return load<DT_F16, LIST>(src, s, w, ws, eps, hold, st);
+    return load<DT_BF16, LIST>(src, s, w, ws, eps, hold, st);
 }
 
-// how many of `left` steps one X X' serves: while a^steps stays below 64 (fp32 results) or 512
-int group_steps(float a, int left, int out_dtype) {
-    const double by = fabs((double)a), limit = out_dtype == YH_F32 ? 64.0 : 512.0;
-    int len = 1;
-    for (double grown = by * by; len < left && grown <= limit; grown *= by) ++len;
-    return len;
+// The steps in groups, each on one X X'.  A singular value s of X becomes s (a + b s^2 + c s^4): from all of [0, 1] that gives
+// the largest one before every step, and the largest factor of every step.  A group ends where the product of its factors
+// would pass 64 (fp32 results) or 511 (16-bit results, S within its range).
+struct Steps {
+    NsHold hold;
+    int len[NS_MAX_GROUPS];
+};
+constexpr double kMostA = 120.0;     // of A, R and T: fp16 at their scales ends at 127
+
+// the power of two above x
+inline short above(double x) { return (short)(x > 1e-30 ? ilogb(x) + 1 : -99); }
+
+// false: coefficients and steps whose matrices would leave fp16's range
+bool steps_in_groups(double a, double b, double c, int steps, int out_dtype, double scale, Steps& p) {
+    const double limit = out_dtype == YH_F32 ? 64.0 : 511.0;
+    double top = 1.0, growth = 1.0, within = 1.0;
+    bool full = true;
+    p.hold.groups = 0;
+    p.hold.scale = scale;
+    for (int j = 0; j < steps; ++j) {
+        const double most = top * top;                               // of A
+        double r = fabs(b * most + c * most * most);                 // of |R|, and of |a + R|
+        double factor = fmax(fabs(a), fabs(a + b * most + c * most * most));
+        const double z = c != 0.0 ? -b / (2.0 * c) : -1.0;
+        if (z > 0.0 && z < most) {
+            r = fmax(r, fabs(b * z / 2.0));
+            factor = fmax(factor, fabs(a + b * z / 2.0));
+        }
+        if (!(most <= kMostA && r <= kMostA && factor * most <= kMostA)) return false;
+        if (full || within * factor > limit) {
+            p.hold.growth[p.hold.groups] = above(growth);
+            p.hold.top[p.hold.groups] = above(top);
+            p.len[p.hold.groups++] = 0;
+            within = 1.0;
+        }
+        within *= factor;
+        growth *= factor;
+        full = within > limit;
+        ++p.len[p.hold.groups - 1];
+        // the largest s (a + b s^2 + c s^4): at the end or where a + 3 b z + 5 c z^2 = 0 (z = s^2)
+        auto at = [&](double x) { return x > 0.0 && x <= most ? sqrt(x) * fabs(a + b * x + c * x * x) : 0.0; };
+        double next = at(most);
+        if (c != 0.0) {
+            const double d = 9.0 * b * b - 20.0 * a * c;
+            if (d >= 0.0) next = fmax(next, fmax(at((-3.0 * b + sqrt(d)) / (10.0 * c)), at((-3.0 * b - sqrt(d)) / (10.0 * c))));
+        } else if (b != 0.0) next = fmax(next, at(-a / (3.0 * b)));
+        top = next;
+    }
+    return true;
 }
 
 // X in fp16 alone: 16-bit numbers, all steps on one X X', and enough of them to pay for the launch that lays S out in
 // planes (a call in us, split / half: 192x576 85.6 / 90.1, 512x512 113 / 117, 256x4096 104.5 / 102.3, 512x2304 129 / 127,
 // 4x512x2304 202 / 195, 1470x4096 475 / 443, 4x1024x9216 897 / 740, 4096x50,176 9520 / 7210)
-bool half_for(const NsShape& s, int g_dtype, int out_dtype, float a, int steps) {
-    return g_dtype != YH_F32 && out_dtype != YH_F32 && s.l > 128 && (double)s.l * (double)s.n * s.count >= 1e6 &&
-           group_steps(a, steps, out_dtype) == steps;
+bool half_for(const NsShape& s, int g_dtype, int out_dtype, const Steps& plan) {
+    return g_dtype != YH_F32 && out_dtype != YH_F32 && s.l > 128 && plan.hold.groups == 1 &&
+           (double)s.l * (double)s.n * s.count >= 1e6;
 }
 
-// G is in the workspace as X and X' (of norm `scale`, their factor beside them); the steps, and the result to `sink`
-int run_steps(const NsShape& s, const Layout& w, char* ws, double scale, float a, float b, float c, int steps, const Sink& sink,
+// G is in the workspace as X and X', factors beside them; the steps, and the result to `sink`
+int run_steps(const NsShape& s, const Layout& w, char* ws, float a, float b, float c, const Steps& plan, const Sink& sink,
               hipStream_t st) {
     char *A = ws + w.a, *T = ws + w.t, *R[2] = {ws + w.r0, ws + w.r1}, *S[2] = {ws + w.s0, ws + w.s1};
     char *X = ws + w.x, *Xt = ws + w.xt, *Xt_next = ws + w.xt2;
     const int lb = (int)(s.lk / 32);
-    const float* factor = (const float*)(ws + w.factor);
-    double rest = 1.0, held = scale;           // X_j = rest * factor * (what is held), which has grown from norm `held`
     NsProducts base = {};
     base.l = s.l;
     base.lk = s.lk;
@@ -299,16 +341,17 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, double scale, float a
         p.blocks = lb;
         return p;
     };
-    int done = 0;
-    while (done < steps) {
-        const int len = group_steps(a, steps - done, sink.dtype);
+    for (int group = 0; group < plan.hold.groups; ++group) {
+        const int len = plan.len[group];
+        const bool last_group = group + 1 == plan.hold.groups;
+        const float* factor = (const float*)(ws + w.factor) + (size_t)group * s.count;
         // A = X X'
         NsProducts gram = base;
         gram.tiles = w.tiles;
         gram.slices = w.slices;
         gram.per_slice = w.per_slice;
         gram.partial = (float*)(ws + w.partial);
-        gram.job[0] = job(X, X, A, (float)(kScaleA * rest * rest), nullptr, 0.0f, nullptr, 0.0f);
+        gram.job[0] = job(X, X, A, kScaleA, nullptr, 0.0f, nullptr, 0.0f);
         gram.job[0].factor = factor;
         gram.job[0].p_mat = w.x_mat;
         gram.job[0].ldp = w.half ? s.nh * 2 : s.nk * 4;
@@ -361,7 +404,6 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, double scale, float a
                 if (const int rc = products(w.square, three, 1, st)) return rc;
             }
         }
-        done += len;
         NsApply ap = {};
         ap.S = Q;
         ap.X = X;
@@ -370,22 +412,16 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, double scale, float a
         ap.x_mat = w.x_mat;
         ap.xt_mat = w.xt_mat;
         ap.sh = s;
-        // what is held next: as large as the growth of `done` steps leaves room for below fp16's largest number
-        double next = ldexp(1.0, (int)floor(log2(32768.0 / pow(fabs((double)a) < 1.0 ? 1.0 : fabs((double)a), (double)done))));
-        if (next < 1.0) next = 1.0;
-        const double k = done < steps ? next / held : rest;
-        ap.factor = factor;
-        ap.k0 = (float)(k / sq);
-        ap.k1 = (float)(k * q);
-        if (done < steps) {
+        ap.factor = last_group ? factor : (const float*)(ws + w.hop) + (size_t)(group + 1) * s.count;
+        ap.k0 = (float)(1.0 / sq);
+        ap.k1 = (float)q;
+        if (!last_group) {
             ap.Yn = X;
             ap.Yt = Xt_next;
             if (const int rc = apply<DT_F32, NS_OUT_SPLIT, false>(ap, st)) return rc;
             char* swap = Xt;
             Xt = Xt_next;
             Xt_next = swap;
-            rest *= held / next;
-            held = next;
         } else if (sink.params) {
             bool on16 = (s.cols * (int64_t)dtype_bytes(sink.dtype)) % 16 == 0;
             for (int i = 0; i < s.count; ++i) {
@@ -448,23 +484,24 @@ int yh_orthogonalize(const void* g, int g_dtype, int64_t g_stride, int64_t ldg, 
     if (count == 0) return YH_OK;
     if (!g || !out) return YH_ERR_NULL;
     const NsShape s = shape_of(rows, cols, (int)count);
-    const Layout w = layout_for(s, half_for(s, g_dtype, out_dtype, a, steps));
     if (!workspace || workspace_bytes < yh_orthogonalize_workspace_bytes(count, rows, cols)) return YH_ERR_WORKSPACE;
     if (!aligned(g, dtype_bytes(g_dtype)) || !aligned(out, dtype_bytes(out_dtype)) || !aligned(workspace, 256)) return YH_ERR_ALIGN;
+    Steps plan;
+    if (!steps_in_groups(a, b, c, steps, out_dtype, first_scale(s), plan)) return YH_ERR_ARG;
+    const Layout w = layout_for(s, half_for(s, g_dtype, out_dtype, plan));
     hipStream_t st = (hipStream_t)stream;
     char* ws = (char*)workspace;
     NsSource src = {};
     src.base = g;
     src.stride_b = g_stride;
     src.stride_r = ldg;
-    const double scale = first_scale(s);
-    if (const int rc = load_as<false>(g_dtype, src, s, w, ws, eps, scale, st)) return rc;
+    if (const int rc = load_as<false>(g_dtype, src, s, w, ws, eps, plan.hold, st)) return rc;
     Sink sink = {};
     sink.dtype = out_dtype;
     sink.out = out;
     sink.out_b = out_stride;
     sink.out_r = ldo;
-    return run_steps(s, w, ws, scale, a, b, c, steps, sink, st);
+    return run_steps(s, w, ws, a, b, c, plan, sink, st);
 }
 
 int yh_muon_step(void* const* params, int p_dtype, const void* const* grads, int g_dtype, float* const* momenta, int count,
@@ -487,21 +524,22 @@ int yh_muon_step(void* const* params, int p_dtype, const void* const* grads, int
         src.buf[i] = momenta[i];
     }
     const NsShape s = shape_of(rows, cols, count);
-    const Layout w = layout_for(s, false);
     if (!workspace || workspace_bytes < yh_orthogonalize_workspace_bytes(count, rows, cols)) return YH_ERR_WORKSPACE;
     if (!aligned(workspace, 256)) return YH_ERR_ALIGN;
+    Steps plan;
+    if (!steps_in_groups(a, b, c, steps, p_dtype, first_scale(s), plan)) return YH_ERR_ARG;
+    const Layout w = layout_for(s, false);
     src.momentum = momentum;
     src.nesterov = nesterov != 0;
     hipStream_t st = (hipStream_t)stream;
     char* ws = (char*)workspace;
-    const double first = first_scale(s);
-    if (const int rc = load_as<true>(g_dtype, src, s, w, ws, eps, first, st)) return rc;
+    if (const int rc = load_as<true>(g_dtype, src, s, w, ws, eps, plan.hold, st)) return rc;
     Sink sink = {};
     sink.dtype = p_dtype;
     sink.params = params;
     sink.decay = (float)(1.0 - (double)lr * (double)weight_decay);
     sink.step = (float)((double)lr * (double)scale);
-    return run_steps(s, w, ws, first, a, b, c, steps, sink, st);
+    return run_steps(s, w, ws, a, b, c, plan, sink, st);
 }
 
 }  // extern "C"

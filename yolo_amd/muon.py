@@ -42,8 +42,9 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coeffs: Tuple[float, float, f
     ``g`` (..., rows, cols), fp32, fp16 or bf16; a matrix taller than wide is worked on transposed.
 
     Columns lie next to each other and rows at any stride of at least ``cols``; leading axes collapse to one.
-    The matrices are held in 22 bits: the result (contiguous, ``out_dtype``) is about 1e-4 off the exact one
-    (3e-5 when it is fp32) before its rounding.  A NaN or an infinity makes its whole matrix NaN.  Forward only."""
+    The matrices are held in 22 bits: the result (contiguous, ``out_dtype``) is within about 2e-4 of the exact
+    one (3e-5 when it is fp32) before its rounding.  Coefficients and steps under which singular values would grow
+    out of range (past 10) are refused.  A NaN or an infinity makes its whole matrix NaN.  Forward only."""
     if not isinstance(g, torch.Tensor):
         raise TypeError(f"g: expected a torch.Tensor, got {type(g).__name__}")
     if not g.is_cuda:
@@ -143,6 +144,16 @@ class Muon(torch.optim.Optimizer):
             for p in group["params"]:
                 if p.dim() < 2:
                     raise ValueError(f"Muon: a parameter of shape {tuple(p.shape)}; weights of two or more axes only")
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # torch has cast the momenta to the types of their weights
+        keys = [key for group in state_dict["param_groups"] for key in group["params"]]
+        weights = [p for group in self.param_groups for p in group["params"]]
+        for key, p in zip(keys, weights):
+            saved = state_dict["state"].get(key, {}).get("momentum_buffer")
+            if saved is not None:
+                self.state[p]["momentum_buffer"] = saved.detach().to(p.device, torch.float32, copy=True).contiguous()
 
     @torch.no_grad()
     def step(self, closure=None):
