@@ -123,9 +123,6 @@ inline bool stages_itself(int x_dtype, int64_t M, int64_t N, int64_t blocks) {
     if (((M + kRows - 1) / kRows) * ((N + 15) / 16) > 256) return M <= kRows && M * blocks <= 96;
     return x_dtype == YH_I8 ? rows * blocks <= 512 && M <= kRows : blocks <= 512 && (M == 1 || rows * blocks <= 96);
 }
-inline size_t workspace_of(const Plan& p, int x_dtype, int64_t M, int64_t N) {
-    return stages_itself(x_dtype, M, N, p.blocks) ? 0 : p.total;
-}
 
 template <int DTX, int DT, bool STAGE>
 int few_rows(const LinearI8Args& a, const void* x, int64_t ldx, int K, hipStream_t st) {
@@ -190,7 +187,7 @@ int yh_quantize_rows(const void* x, int x_dtype, int64_t ldx, int8_t* q, int64_t
 
 size_t yh_linear_i8_workspace_bytes(int x_dtype, int64_t M, int64_t N, int64_t K) {
     if (check_sizes(M, N, K) != YH_OK || M == 0 || N == 0) return 0;
-    return workspace_of(plan_for(M, N, K), x_dtype, M, N);
+    return stages_itself(x_dtype, M, N, (K + 127) / 128) ? 0 : plan_for(M, N, K).total;
 }
 
 int yh_linear_i8(const void* x, int x_dtype, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw,
@@ -202,9 +199,11 @@ int yh_linear_i8(const void* x, int x_dtype, int64_t ldx, const float* x_scale, 
     if ((x_dtype == YH_I8) != (x_scale != nullptr)) return YH_ERR_ARG;
     if (M == 0 || N == 0) return YH_OK;
     if (!x || !w || !w_scale || !y) return YH_ERR_NULL;
-    const Plan p = plan_for(M, N, K);
-    const size_t need = workspace_of(p, x_dtype, M, N);
-    if (need && (!workspace || workspace_bytes < need)) return YH_ERR_WORKSPACE;
+    const bool itself = stages_itself(x_dtype, M, N, (K + 127) / 128);
+    Plan p = {};
+    if (itself) p.blocks = (int)((K + 127) / 128);
+    else p = plan_for(M, N, K);
+    if (p.total && (!workspace || workspace_bytes < p.total)) return YH_ERR_WORKSPACE;
     if (!aligned(x, dtype_bytes(x_dtype)) || !aligned(x_scale, 4) || !aligned(w, 16) || ldw % 16 != 0 ||
         !aligned(w_scale, 4) || !aligned(bias, 4) || !aligned(y, dtype_bytes(y_dtype)) || !aligned(workspace, 256))
         return YH_ERR_ALIGN;
@@ -231,7 +230,7 @@ int yh_linear_i8(const void* x, int x_dtype, int64_t ldx, const float* x_scale, 
     a.tiles_n = p.tiles_n;
     const size_t e = dtype_bytes(y_dtype);
     a.store = (ldy * e) % 16 == 0 && aligned(y, 16) ? STORE_16 : ldy % 2 == 0 && aligned(y, 2 * e) ? STORE_PAIR : STORE_ONE;
-    if (need == 0) {
+    if (itself) {
         a.sx = x_scale;
         if (y_dtype == YH_F32) return few_rows_of<DT_F32>(a, x, x_dtype, ldx, (int)K, st);
         if (y_dtype == YH_F16) return few_rows_of<DT_F16>(a, x, x_dtype, ldx, (int)K, st);

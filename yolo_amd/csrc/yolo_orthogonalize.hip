@@ -102,7 +102,7 @@ Layout layout_for(const NsShape& s, bool half) {
     for (int k = 0; k < TILE_KINDS; ++k) {
         const int t = triangle_tiles(s.l, kTiles[k].bm);
         const int64_t wgs = (int64_t)t * s.count;
-        for (int cut = 1; cut <= 16 && cut * 4 <= blocks + 3; cut *= 2) {
+        for (int cut = 1; cut <= 16 && cut * 4 <= blocks + 3; ++cut) {
             if (cut > 1 && wgs * cut > 4096) break;
             const int64_t per = (blocks + cut - 1) / cut;
             double us = tile_time(kTiles[k], wgs * cut, per);
