@@ -79,7 +79,7 @@ struct Layout {
     int norm_blocks;
     bool half;
     int gram, tiles, slices, per_slice;      // X X': kind of tile, tiles on and below the diagonal, slices
-    int square, square_tiles;                // the l x l products
+    int square[2], square_tiles[2];          // the l x l products, one or two in a launch
 };
 
 inline int triangle_tiles(int64_t l, int b) {
@@ -98,7 +98,7 @@ Layout layout_for(const NsShape& s, bool half) {
     w.sq_mat = s.l * s.lk * 4;
     // the contraction of X X' is cut when the tiles alone do not fill the card
     const int64_t blocks = half ? s.nh / 64 : s.nk / 32;
-    double best = 0.0, best_square = 0.0;
+    double best = 0.0, best_square[2] = {0.0, 0.0};
     for (int k = 0; k < TILE_KINDS; ++k) {
         const int t = triangle_tiles(s.l, kTiles[k].bm);
         const int64_t wgs = (int64_t)t * s.count;
@@ -115,11 +115,13 @@ Layout layout_for(const NsShape& s, bool half) {
                 w.slices = (int)((blocks + per - 1) / per);
             }
         }
-        const double us = tile_time(kTiles[k], wgs, s.lk / 32);
-        if (best_square == 0.0 || us < best_square) {
-            best_square = us;
-            w.square = k;
-            w.square_tiles = t;
+        for (int two = 0; two < 2; ++two) {
+            const double us = tile_time(kTiles[k], wgs * (two + 1), s.lk / 32);
+            if (best_square[two] == 0.0 || us < best_square[two]) {
+                best_square[two] = us;
+                w.square[two] = k;
+                w.square_tiles[two] = t;
+            }
         }
     }
     size_t off = 0;
@@ -323,7 +325,7 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, float a, float b, flo
     base.l = s.l;
     base.lk = s.lk;
     base.count = s.count;
-    base.tiles = w.square_tiles;
+    base.tiles = w.square_tiles[0];
     base.slices = 1;
     base.per_slice = lb;
     auto job = [&](const char* P, const char* Q, char* out, float k0, const char* E1, float k1, const char* E2, float k2) {
@@ -382,7 +384,7 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, float a, float b, flo
             char* Rj = R[j & 1];
             NsProducts one = base;
             one.job[0] = job(A, A, Rj, c * kScaleR / (kScaleA * kScaleA), A, b * kScaleR / kScaleA, nullptr, 0.0f);
-            if (const int rc = products(w.square, one, 1, st)) return rc;
+            if (const int rc = products(w.square[0], one, 1, st)) return rc;
             int jobs = 0;
             NsProducts two = base;
             const bool last = j + 1 == len;
@@ -396,12 +398,14 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, float a, float b, flo
                 Q = Rj;
                 sq = kScaleR;
             }
-            if (jobs)
-                if (const int rc = products(w.square, two, jobs, st)) return rc;
+            if (jobs) {
+                two.tiles = w.square_tiles[jobs - 1];
+                if (const int rc = products(w.square[jobs - 1], two, jobs, st)) return rc;
+            }
             if (!last) {
                 NsProducts three = base;
                 three.job[0] = job(T, Rj, A, 1.0f / kScaleR, T, a, nullptr, 0.0f);
-                if (const int rc = products(w.square, three, 1, st)) return rc;
+                if (const int rc = products(w.square[0], three, 1, st)) return rc;
             }
         }
         NsApply ap = {};
