@@ -85,6 +85,18 @@ def test_16_bit_gradients(dev, rows, cols, count, g_dtype, out):
     assert torch.equal(got[4], got[0]) and not got[1].any() and torch.isnan(got[2:4]).all()
 
 
+@pytest.mark.parametrize("rows,cols,count", [(130, 150, 48), (263, 263, 48), (330, 326, 32), (326, 330, 64), (1150, 2500, 2)])
+def test_every_tile_of_the_products(dev, rows, cols, count):
+    """Batches that fill the card with each of the tiles the products are cut into."""
+    gen = torch.Generator().manual_seed(count)
+    g = torch.randn(count, rows, cols, generator=gen)
+    for dtype, out in ((torch.float32, torch.float32), (torch.float32, torch.bfloat16), (torch.float16, torch.float16)):
+        typed = g.to(dtype)
+        got = orthogonalize(typed.to(dev), out_dtype=out)
+        for i in (0, count // 2, count - 1):
+            assert off(got[i], polar(typed[i])) <= FAR[out], (dtype, out, i)
+
+
 @pytest.mark.parametrize("steps", [1, 2, 3, 4, 6, 7, 9])
 @pytest.mark.parametrize("rows,cols", [(40, 100), (100, 40), (130, 260)])
 def test_any_number_of_steps(dev, rows, cols, steps):

@@ -21,17 +21,17 @@ inline size_t dtype_bytes(int dt) { return dt == YH_F32 ? 4 : 2; }
 constexpr int64_t kMaxShort = 32768, kMaxLong = (int64_t)1 << 24, kMaxNumbers = (int64_t)1 << 38;
 // Tiles of the products: us for a block of 32 numbers of the contraction with one workgroup on a CU, and for each more that
 // fits; `start` us to begin and end.  The choice is the least time of its rounds over the 256 CUs.
-// Symmetric products (us, 192 / 128 / 64 / 32;
-// l = contraction unless stated, matrices in brackets): 192 22 / 9.9 / 6.2 / 4.4, 512 (4) 31 / 15 / 8.9 / 8.6, 1024 44 / 22 / 12.1 /
-// 12.2, 1024 (4) 49 / 26 / 28 / 33, 1470 59 / 30 / 21 / 30, 2048 77 / 41 / 46 / 77, 4096 183 / 239 / 339 / -, 4096 over 50,176
-// 1974 / 2521 / 4531 / -: 4096 is 253 tiles of 192, one for each CU, but 528 of 128, two and a bit.
+// Symmetric products (us, 192 / 128 / 96 / 64 / 32; l = contraction unless stated, matrices in brackets): 192 22 / 9.9 / 12.8 / 6.2 /
+// 4.4, 512 (4) 31 / 15 / 17.7 / 8.9 / 8.6, 1024 44 / 22 / 23 / 12.1 / 12.2, 1024 (4) 49 / 26 / 34 / 28 / 33, 1470 59 / 30 / 31 / 21 / 30,
+// 2048 77 / 41 / 43 / 46 / 77, 2048 (2) - / 83 / 67 / 80 / -, 4096 183 / 239 / 238 / 339 / -, 4096 over 50,176 1974 / 2521 / - / 4531 / -:
+// 4096 is 253 tiles of 192, one for each CU, but 528 of 128, two and a bit; two of 2048 are 506 tiles of 96, two for each.
 struct TileKind {
     int bm, bn, per_cu;
     double block, more, start;
 };
-enum { TILE_LARGE = 0, TILE_128 = 1, TILE_64 = 2, TILE_32 = 3, TILE_KINDS = 4 };
-constexpr TileKind kTiles[TILE_KINDS] = {
-    {192, 192, 1, 1.30, 0.0, 6.0}, {128, 128, 1, 0.58, 0.0, 4.3}, {64, 64, 2, 0.23, 0.14, 4.3}, {32, 32, 5, 0.10, 0.11, 3.8}};
+enum { TILE_LARGE = 0, TILE_128 = 1, TILE_64 = 2, TILE_32 = 3, TILE_KINDS = 4, TILE_96 = 4, PRODUCT_KINDS = 5 };
+constexpr TileKind kTiles[PRODUCT_KINDS] = {
+    {192, 192, 1, 1.30, 0.0, 6.0}, {128, 128, 1, 0.58, 0.0, 4.3}, {64, 64, 2, 0.23, 0.14, 4.3}, {32, 32, 5, 0.10, 0.11, 3.8}, {96, 96, 2, 0.60, 0.375, 4.3}};
 // Y = q X + S X (us, 128x256 / 128 / 64 / 32): 64 x 9000 9.5 / 6.5 / 4.8 / 5.0, 192 x 576 13.4 / 8.4 / 5.0 / 4.3, 512 x 2304 (4)
 // 25.7 / 30.0 / 24.6 / 32.0, 1024 x 9216 (4) 232 / 265 / 330 / 573, 1470 x 4096 52 / 59 / 70 / 153, 4096 x 50,176 3869 / 4547 /
 // 7632 / 13944 (256x128: 4078); written over X in split form 1024 x 9216 (4) 310 / 298 / 385 / 615.
@@ -99,7 +99,7 @@ Layout layout_for(const NsShape& s, bool half) {
     // the contraction of X X' is cut when the tiles alone do not fill the card
     const int64_t blocks = half ? s.nh / 64 : s.nk / 32;
     double best = 0.0, best_square[2] = {0.0, 0.0};
-    for (int k = 0; k < TILE_KINDS; ++k) {
+    for (int k = 0; k < PRODUCT_KINDS; ++k) {
         const int t = triangle_tiles(s.l, kTiles[k].bm);
         const int64_t wgs = (int64_t)t * s.count;
         for (int cut = 1; cut <= 16 && cut * 4 <= blocks + 3; ++cut) {
@@ -205,6 +205,7 @@ template <class Math>
 int products_in(int kind, const NsProducts& a, int jobs, hipStream_t st) {
     if (kind == TILE_LARGE) return products_of<Math, 192, 2, 4, 3>(a, jobs, st);
     if (kind == TILE_128) return products_of<Math, 128, 2, 4, 4>(a, jobs, st);
+    if (kind == TILE_96) return products_of<Math, 96, 2, 2, 3>(a, jobs, st);
     if (kind == TILE_64) return products_of<Math, 64, 2, 2, 4>(a, jobs, st);
     return products_of<Math, 32, 2, 2, 4>(a, jobs, st);
 }
