@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from functools import lru_cache
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -21,8 +22,13 @@ _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 COEFFS = (3.4445, -4.7750, 2.0315)      # raises small singular values fastest; they end within 0.7 .. 1.2
 
 
-def _workspace(lib, count: int, rows: int, cols: int, device) -> torch.Tensor:
-    nbytes = lib.yh_orthogonalize_workspace_bytes(count, rows, cols)
+@lru_cache(maxsize=4096)
+def _workspace_bytes(count: int, rows: int, cols: int) -> int:
+    return _lib.load().yh_orthogonalize_workspace_bytes(count, rows, cols)
+
+
+def _workspace(count: int, rows: int, cols: int, device) -> torch.Tensor:
+    nbytes = _workspace_bytes(count, rows, cols)
     if nbytes == 0:
         raise ValueError(f"{count} matrices of {rows} x {cols}: outside the supported range (shorter side up to 32,768, "
                          "longer up to 2^24)")
@@ -66,7 +72,7 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coeffs: Tuple[float, float, f
     batch = g.reshape(-1, rows, cols)
     count = batch.shape[0]
     lib = _lib.load()
-    ws = _workspace(lib, count, rows, cols, g.device)
+    ws = _workspace(count, rows, cols, g.device)
     ld = batch.stride(1) if rows > 1 else cols
     with _on_device(g.device):
         _lib.check(lib.yh_orthogonalize(
@@ -120,7 +126,7 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
     for at in range(0, len(params), most):
         some = slice(at, at + most)
         count = len(params[some])
-        ws = _workspace(lib, count, rows, cols, dev)
+        ws = _workspace(count, rows, cols, dev)
         lists = [(ctypes.c_void_p * count)(*(t.data_ptr() for t in tensors[some])) for tensors in (params, grads, momenta)]
         with _on_device(dev):
             _lib.check(lib.yh_muon_step(
