@@ -214,8 +214,8 @@ __device__ __forceinline__ void half_get_n(const char* p, float (&v)[N]) {
 
 // ---------------------------------------------------------------- G -> X and X', split or half
 // 64 x 64 numbers of G per workgroup; `nat` gets G's own rows, `tra` its columns, both times scale / |G|.  vec: rows
-// of G (and of the momentum) on 16 bytes and of a multiple of eight numbers.  4096 x 50,176 bf16: 518 us for 2.06 GB
-// (4.0 TB/s).
+// of G (and of the momentum) on 16 bytes and of a multiple of eight numbers.  4096 x 50,176 bf16, fp16 alone: 286 us
+// for 1.23 GB (4.3 TB/s); 4 x 1024 x 9216 with momentum, split: 117 us for 528 MB (4.5 TB/s).
 template <int DT, bool LIST, bool HALF>
 __global__ __launch_bounds__(256) void ns_convert_kernel(NsSource src, NsShape sh, const double* __restrict__ parts, int nparts,
                                                          double eps, NsHold hold, char* __restrict__ nat, long long nat_mat,
@@ -651,7 +651,7 @@ __global__ __launch_bounds__((ChainGrid<SIDE, T>::THREADS)) void ns_chain_kernel
     }
 }
 
-// S split -> the planes hi and lo of each row, lh numbers each
+// S split -> the planes hi and lo of each row, lh numbers each.  4096 x 4096: 25 us (134 MB); 4 x 512 x 512: 4 us, a launch.
 static __global__ __launch_bounds__(256) void ns_planes_kernel(const char* __restrict__ S, long long s_mat, char* __restrict__ planes,
                                                                long long planes_mat, NsShape sh) {
     const long long eights = sh.lh / 8, total = sh.l * eights;

@@ -79,7 +79,7 @@ struct TileOperand {
     long long rows;
     long long first;
     long long last_chunk;   // below 2^31
-    int turn = 1 << 30;     // blocks of a row: from there on they are read again from the first
+    int turn = 1 << 30;     // blocks of a row (of B): from there on they are read again from the first
 };
 
 // A workgroup of WM x WN wavefronts computes BM x BN numbers over the blocks [kb0, kb1) of the contraction.
@@ -88,8 +88,8 @@ struct TileOperand {
 //
 // A ring of STAGES blocks in LDS: while one is worked on, the next STAGES - 1 are on their way, straight from memory into
 // LDS (16 bytes a lane, no registers in between; the exchange of chunks is made in the address a lane reads, since a
-// wavefront's 1,024 bytes land in LDS in lane order).  A load takes about 1 us, a block's products 0.2 us (128 x 128) to
-// 0.9 us (256 x 256): what is in flight hides the difference, within a workgroup by stages and on a CU by several
+// wavefront's 1,024 bytes land in LDS in lane order).  A load takes about 1 us, a block's products 0.6 us (128 x 128) to
+// 1.2 us (128 x 256): what is in flight hides the difference, within a workgroup by stages and on a CU by several
 // workgroups.  The stages are distinct objects, so reads of one need not wait for loads into another.  One barrier per
 // block: it says that the block has landed for every wavefront and that the block before it has been read by all.
 template <class Math, int BM, int BN, int WM, int WN, int STAGES, bool ROWS_B>
