@@ -98,6 +98,23 @@ def test_linear_i8_of_quantized_features(dev, m, k, n):
     check(y, xs[:, :k].cpu(), s, w_[:, :k], t, None)
 
 
+@pytest.mark.parametrize("m,k,n,dtype", [(1, 65536, 40, torch.bfloat16), (1, 65537, 40, torch.float32), (1, 131071, 20, torch.float16),
+                                         (3, 4096, 40, torch.float32), (4, 4096, 40, torch.float16), (64, 700, 40, torch.bfloat16),
+                                         (16, 4096, 40, torch.int8), (16, 4097, 40, torch.int8), (1, 65536, 40, torch.int8)])
+def test_on_both_sides_of_what_is_brought_in_on_the_way(dev, m, k, n, dtype):
+    """The largest rows that the product's workgroups bring into LDS themselves, and the first that they do not."""
+    gen = torch.Generator().manual_seed(m + k)
+    w, t = weights(n, k, gen, dev)
+    if dtype == torch.int8:
+        q, s = torch.randint(-128, 128, (m, k), generator=gen, dtype=torch.int8), torch.rand(m, generator=gen)
+        y = linear_i8(q.to(dev), w, t, x_scale=s.to(dev))
+        check(y, q, s.to(dev), w, t, None)
+    else:
+        x = torch.randn(m, k, generator=gen).to(dtype)
+        q, s = quantized(x)
+        check(linear_i8(x.to(dev), w, t, out_dtype=torch.float32), q, s, w, t, None)
+
+
 def test_the_largest_sum_there_is(dev):
     k = 131071
     x = torch.full((2, k + 1), -128, dtype=torch.int8, device=dev)

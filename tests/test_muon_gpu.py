@@ -289,6 +289,54 @@ def test_muon_step_refusals(dev):
         muon_step([p[0]], [p[1]], [p[2]], lr=float("nan"))
 
 
+@pytest.mark.parametrize("rows,cols,count", [(40, 90, 2), (90, 40, 2), (129, 8000, 1), (8000, 129, 1)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_what_lies_between_the_rows_of_the_result_stays(dev, rows, cols, count, dtype):
+    """Results at strides of their own, stored 16 bytes, a pair or one number at a time."""
+    gen = torch.Generator().manual_seed(12)
+    lib, code = _lib.load(), _lib.DTYPE_CODES[dtype]
+    g = torch.randn(count, rows, cols, generator=gen).to(dtype).to(dev)
+    want = orthogonalize(g, out_dtype=dtype)
+    nbytes = lib.yh_orthogonalize_workspace_bytes(count, rows, cols)
+    ws = torch.empty(nbytes + 256, dtype=torch.uint8, device=dev)
+    ws[nbytes:] = 77
+    for ldo, at in ((cols + 8, 0), (cols + 6, 2), (cols + 5, 1)):
+        stride = rows * ldo + 8
+        out = torch.full((count * stride + 64,), 7.0, dtype=dtype, device=dev)
+        _lib.check(lib.yh_orthogonalize(g.data_ptr(), code, rows * cols, cols, out[at:].data_ptr(), code, stride, ldo, count, rows, cols,
+                                        *COEFFS, 5, 1e-7, ws.data_ptr(), nbytes, torch.cuda.current_stream(dev).cuda_stream))
+        inside = torch.zeros_like(out, dtype=torch.bool)
+        for i in range(count):
+            where = ((rows, cols), (ldo, 1), at + i * stride)
+            assert torch.equal(out.as_strided(*where), want[i]), (ldo, i)
+            inside.as_strided(*where).fill_(True)
+        assert (out[~inside] == 7).all(), ldo
+        assert (ws[nbytes:] == 77).all()
+
+
+def test_captured_with_16_bit_gradients(dev):
+    """The form that holds X in fp16 alone, captured and replayed between eager calls."""
+    gen = torch.Generator().manual_seed(13)
+    g = torch.randn(2, 513, 1200, generator=gen).to(torch.bfloat16).to(dev)
+    orthogonalize(g)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = orthogonalize(g)
+    for turn in range(4):
+        g.copy_(torch.randn(g.shape, generator=gen))
+        want = orthogonalize(g)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want), turn
+
+
+def test_under_inference_mode(dev):
+    with torch.inference_mode():
+        p, g, m = (torch.ones(20, 30, device=dev) for _ in range(3))
+        muon_step([p], [g], [m], lr=0.1)
+        assert (p < 1).all() and torch.allclose(m, torch.full_like(m, 1.95))
+
+
 def test_streams_and_captured_graphs(dev):
     gen = torch.Generator().manual_seed(11)
     shapes = [(64, 147), (130, 300), (300, 130)]

@@ -164,3 +164,14 @@ def test_momenta_stay_fp32_through_a_state_dict():
         got, saved = (o.state[p]["momentum_buffer"] for o in (second, first))
         assert got.dtype == torch.float32 and torch.equal(got, saved) and got.data_ptr() != saved.data_ptr()
     assert second.param_groups[0]["lr"] == 0.02
+
+
+def test_the_first_step_of_a_weight_is_not_captured(monkeypatch):
+    """A replay would set the momentum back to zero each time."""
+    w = torch.nn.Parameter(torch.zeros(3, 5))
+    w.grad = torch.ones(3, 5)
+    optim = Muon([w])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before the capture"):
+        optim.step()
+    assert not optim.state[w]

@@ -134,7 +134,8 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
                 float(lr), float(momentum), int(bool(nesterov)), float(weight_decay), float(scale), *(float(v) for v in coeffs),
                 int(steps), float(eps), ws.data_ptr(), ws.numel(), _stream(dev)))
     for t in (*params, *momenta):
-        torch.autograd.graph.increment_version(t)
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
 
 
 class Muon(torch.optim.Optimizer):
@@ -174,6 +175,9 @@ class Muon(torch.optim.Optimizer):
                     continue
                 state = self.state[p]
                 if "momentum_buffer" not in state:
+                    if torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("Muon: the first step of a weight makes its momentum, and a captured graph would clear it "
+                                           "in every replay; take one step before the capture")
                     state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 alike.setdefault((tuple(p.shape), p.dtype, p.grad.dtype, p.device), []).append(p)
             for ps in alike.values():
