@@ -187,6 +187,18 @@ def test_coefficients_within_range(dev, coeffs, steps):
         assert off(got, polar(g, steps, coeffs)) <= 1e-4
 
 
+def test_coefficients_out_of_range_name_themselves(dev):
+    x = torch.randn(8, 16, device=dev)
+    before = x.clone()
+    with pytest.raises(ValueError, match="coefficients"):
+        orthogonalize(x, coeffs=(3.0, -4.0, 2.0))
+    with pytest.raises(ValueError, match="coefficients"):
+        muon_step([x], [x.clone()], [x.clone()], lr=0.1, coeffs=(30.0, 0.0, 0.0))
+    with pytest.raises(ValueError, match="finite"):
+        muon_step([x], [x.clone()], [x.clone()], lr=math.nan)
+    assert torch.equal(x, before)
+
+
 def test_state_dict_of_16_bit_weights(dev):
     torch.manual_seed(1)
     w = torch.nn.Parameter(torch.randn(24, 40, device=dev, dtype=torch.bfloat16))

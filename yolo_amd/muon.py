@@ -42,6 +42,13 @@ def _check_steps(steps: int, eps: float) -> None:
         raise ValueError(f"eps: expected a finite number that is not negative, got {eps}")
 
 
+def _check(rc: int) -> None:
+    if rc == _lib.YH_ERR_ARG:
+        raise ValueError("coeffs: coefficients under which so many steps leave the supported range (singular values past 10), or a "
+                         "number that is not finite")
+    _lib.check(rc)
+
+
 def orthogonalize(g: torch.Tensor, steps: int = 5, coeffs: Tuple[float, float, float] = COEFFS, eps: float = 1e-7,
                   out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``steps`` times ``X <- (a + b X X' + c (X X')^2) X`` from ``X = g / (|g| + eps)`` for every matrix of
@@ -75,7 +82,7 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coeffs: Tuple[float, float, f
     ws = _workspace(count, rows, cols, g.device)
     ld = batch.stride(1) if rows > 1 else cols
     with _on_device(g.device):
-        _lib.check(lib.yh_orthogonalize(
+        _check(lib.yh_orthogonalize(
             batch.data_ptr(), _lib.DTYPE_CODES[g.dtype], batch.stride(0) if count > 1 else rows * ld, ld, out.data_ptr(),
             _lib.DTYPE_CODES[out_dtype], rows * cols, cols, count, rows, cols, *(float(v) for v in coeffs), int(steps),
             float(eps), ws.data_ptr(), ws.numel(), _stream(g.device)))
@@ -129,7 +136,7 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
         ws = _workspace(count, rows, cols, dev)
         lists = [(ctypes.c_void_p * count)(*(t.data_ptr() for t in tensors[some])) for tensors in (params, grads, momenta)]
         with _on_device(dev):
-            _lib.check(lib.yh_muon_step(
+            _check(lib.yh_muon_step(
                 lists[0], _lib.DTYPE_CODES[first.dtype], lists[1], _lib.DTYPE_CODES[grads[0].dtype], lists[2], count, rows, cols,
                 float(lr), float(momentum), int(bool(nesterov)), float(weight_decay), float(scale), *(float(v) for v in coeffs),
                 int(steps), float(eps), ws.data_ptr(), ws.numel(), _stream(dev)))
