@@ -190,11 +190,11 @@ def test_coefficients_within_range(dev, coeffs, steps):
 def test_coefficients_out_of_range_name_themselves(dev):
     x = torch.randn(8, 16, device=dev)
     before = x.clone()
-    with pytest.raises(ValueError, match="coefficients"):
+    with pytest.raises(_lib.YoloHeadError, match="coefficients"):
         orthogonalize(x, coeffs=(3.0, -4.0, 2.0))
-    with pytest.raises(ValueError, match="coefficients"):
+    with pytest.raises(_lib.YoloHeadError, match="coefficients"):
         muon_step([x], [x.clone()], [x.clone()], lr=0.1, coeffs=(30.0, 0.0, 0.0))
-    with pytest.raises(ValueError, match="finite"):
+    with pytest.raises(_lib.YoloHeadError, match="finite"):
         muon_step([x], [x.clone()], [x.clone()], lr=math.nan)
     assert torch.equal(x, before)
 

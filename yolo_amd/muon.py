@@ -44,8 +44,8 @@ def _check_steps(steps: int, eps: float) -> None:
 
 def _check(rc: int) -> None:
     if rc == _lib.YH_ERR_ARG:
-        raise ValueError("coeffs: coefficients under which so many steps leave the supported range (singular values past 10), or a "
-                         "number that is not finite")
+        raise _lib.YoloHeadError(rc, "coeffs: coefficients under which so many steps leave the supported range (singular values "
+                                     "past 10), or a number that is not finite")
     _lib.check(rc)
 
 
