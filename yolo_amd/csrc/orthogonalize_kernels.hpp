@@ -337,11 +337,12 @@ struct NsProduct {
     const float* factor;            // of each matrix, or null: k0 times its square
     float k0, k1, k2;
     int blocks;                     // of 128 bytes along the contraction
+    int first, tiles;               // of the tiles on and below the diagonal: this job's
 };
 struct NsProducts {
-    NsProduct job[2];
+    NsProduct job[2];               // the second may have no tiles
     long long l, lk;
-    int count, tiles;               // tiles on and below the diagonal
+    int count;
     int slices, per_slice;          // the contraction in slices, when partial sums are joined
     float* partial;
 };
@@ -416,14 +417,17 @@ template <class Math, int BM, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(64 * WM * WN, 2) void ns_product_kernel(NsProducts a) {
     typedef TileProduct<Math, BM, BM, WM, WN, STAGES, true> T;
     YH_TILE_RING(T)
-    const NsProduct p = a.job[blockIdx.y];
-    const long long per = (long long)a.tiles * a.count;
-    const long long id = xcd_order(blockIdx.x, per * a.slices);
+    const long long before = (long long)a.job[0].tiles * a.count * a.slices;
+    long long id = xcd_order(blockIdx.x, before + (long long)a.job[1].tiles * a.count);      // slices only of a job by itself
+    const int second = id >= before;
+    const NsProduct p = a.job[second];
+    if (second) id -= before;
+    const long long per = (long long)p.tiles * a.count;
     const int slice = (int)(id / per);
     const long long mt = id - slice * per;
-    const long long mat = mt / a.tiles;
+    const long long mat = mt / p.tiles;
     int ti, tj;
-    triangle((int)(mt - mat * a.tiles), ti, tj);
+    triangle(p.first + (int)(mt - mat * p.tiles), ti, tj);
     typename T::Acc acc[T::TM][T::TN] = {};
     const TileOperand A = {p.P + mat * p.p_mat, p.ldp, a.l, (long long)ti * BM, p.ldp - 16};
     const TileOperand B = {p.Q + mat * p.p_mat, p.ldp, a.l, (long long)tj * BM, p.ldp - 16};
@@ -451,11 +455,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_join_kernel(NsProducts a) 
     typedef TileProduct<MathSplit, BM, BM, WM, WN, STAGES, true> T;
     __shared__ __align__(16) char lds[T::WAVES * TURN_BYTES<T::TN>];
     const NsProduct p = a.job[0];
-    const long long per = (long long)a.tiles * a.count;
+    const long long per = (long long)p.tiles * a.count;
     const long long mt = blockIdx.x;
-    const long long mat = mt / a.tiles;
+    const long long mat = mt / p.tiles;
     int ti, tj;
-    triangle((int)(mt - mat * a.tiles), ti, tj);
+    triangle((int)(mt - mat * p.tiles), ti, tj);
     const int wave = threadIdx.x >> 6;
     const float* part = a.partial + mt * (BM * BM) + threadIdx.x * 4;
     typename T::Acc acc[T::TM][T::TN] = {};

@@ -38,11 +38,14 @@ constexpr TileKind kTiles[PRODUCT_KINDS] = {
 constexpr TileKind kApplyTiles[TILE_KINDS] = {
     {128, 256, 1, 1.18, 0.0, 4.0}, {128, 128, 1, 0.69, 0.0, 4.3}, {64, 64, 2, 0.25, 0.18, 4.3}, {32, 32, 5, 0.10, 0.13, 3.8}};
 
-// us for `wgs` workgroups of `blocks` blocks each
+// us for `wgs` workgroups of `blocks` blocks each: their rounds, or what they take in at 14 TB/s (the caches: 1056 workgroups of 64 over
+// 64 blocks 79.5 us, 1128 over 94 138, 2080 over 128 340)
 double tile_time(const TileKind& k, int64_t wgs, int64_t blocks) {
     const int64_t at_once = 256 * (int64_t)k.per_cu;
     const int64_t together = wgs >= at_once ? k.per_cu : (wgs + 255) / 256;
-    return (double)((wgs + at_once - 1) / at_once) * ((double)blocks * (k.block + k.more * (double)(together - 1)) + k.start);
+    const double rounds = (double)((wgs + at_once - 1) / at_once) * ((double)blocks * (k.block + k.more * (double)(together - 1)) + k.start);
+    const double intake = (double)(wgs * blocks) * (double)((k.bm + k.bn) * TILE_BLOCK_BYTES) / 14e6;
+    return rounds > intake ? rounds : intake;
 }
 
 // powers of two the split matrices are held at: A, R and T up to 120, S up to 1022 (steps_in_groups)
@@ -79,7 +82,8 @@ struct Layout {
     int norm_blocks;
     bool half;
     int gram, tiles, slices, per_slice;      // X X': kind of tile, tiles on and below the diagonal, slices
-    int square[2], square_tiles[2];          // the l x l products, one or two in a launch
+    int square, square_tiles;                // an l x l product by itself
+    int shared, shared_tiles, shares;        // and with a share of S: of how many
 };
 
 inline int triangle_tiles(int64_t l, int b) {
@@ -98,7 +102,7 @@ Layout layout_for(const NsShape& s, bool half) {
     w.sq_mat = s.l * s.lk * 4;
     // the contraction of X X' is cut when the tiles alone do not fill the card
     const int64_t blocks = half ? s.nh / 64 : s.nk / 32;
-    double best = 0.0, best_square[2] = {0.0, 0.0};
+    double best = 0.0, best_square = 0.0, best_shared = 0.0;
     for (int k = 0; k < PRODUCT_KINDS; ++k) {
         const int t = triangle_tiles(s.l, kTiles[k].bm);
         const int64_t wgs = (int64_t)t * s.count;
@@ -115,12 +119,26 @@ Layout layout_for(const NsShape& s, bool half) {
                 w.slices = (int)((blocks + per - 1) / per);
             }
         }
-        for (int two = 0; two < 2; ++two) {
-            const double us = tile_time(kTiles[k], wgs * (two + 1), s.lk / 32);
-            if (best_square[two] == 0.0 || us < best_square[two]) {
-                best_square[two] = us;
-                w.square[two] = k;
-                w.square_tiles[two] = t;
+        const double us = tile_time(kTiles[k], wgs, s.lk / 32);
+        if (best_square == 0.0 || us < best_square) {
+            best_square = us;
+            w.square = k;
+            w.square_tiles = t;
+        }
+    }
+    // S of a step is not needed before the next step's: it goes along with T alone, or in shares with T, the next A and the next R,
+    // so that a launch fills the card without beginning another round (a call in us, with T alone / as chosen: 1470x4096 440 / 425,
+    // 1024x1024 225 / 205, four of them 497 / 447, 2048x2048 754 / 700, 3000x5000 2380 / 2007, 512x512 115 / 116)
+    for (int k = 0; k < PRODUCT_KINDS; ++k) {
+        const int t = triangle_tiles(s.l, kTiles[k].bm);
+        for (int shares = 1; shares <= 3; ++shares) {
+            const double us = shares * tile_time(kTiles[k], (int64_t)(t + (t + shares - 1) / shares) * s.count, s.lk / 32) +
+                              (3 - shares) * best_square;
+            if (best_shared == 0.0 || us < best_shared) {
+                best_shared = us;
+                w.shared = k;
+                w.shared_tiles = t;
+                w.shares = shares;
             }
         }
     }
@@ -192,25 +210,23 @@ int apply_half(int dt, bool tall, const NsApply& a, hipStream_t st) {
 }
 
 template <class Math, int BM, int WM, int WN, int STAGES>
-int products_of(const NsProducts& a, int jobs, hipStream_t st) {
-    const unsigned grid = (unsigned)((int64_t)a.tiles * a.count * a.slices);
-    hipLaunchKernelGGL((ns_product_kernel<Math, BM, WM, WN, STAGES>), dim3(grid, (unsigned)jobs), dim3(64 * WM * WN), 0, st, a);
+int products_of(const NsProducts& a, hipStream_t st) {
+    const unsigned grid = (unsigned)(((int64_t)a.job[0].tiles * a.slices + a.job[1].tiles) * a.count);
+    hipLaunchKernelGGL((ns_product_kernel<Math, BM, WM, WN, STAGES>), dim3(grid), dim3(64 * WM * WN), 0, st, a);
     if (const int rc = launch_status()) return rc;
     if (a.slices > 1)
-        hipLaunchKernelGGL((ns_join_kernel<BM, WM, WN, STAGES>), dim3((unsigned)(a.tiles * a.count)), dim3(64 * WM * WN), 0, st, a);
+        hipLaunchKernelGGL((ns_join_kernel<BM, WM, WN, STAGES>), dim3((unsigned)(a.job[0].tiles * a.count)), dim3(64 * WM * WN), 0, st, a);
     return launch_status();
 }
 
 template <class Math>
-int products_in(int kind, const NsProducts& a, int jobs, hipStream_t st) {
-    if (kind == TILE_LARGE) return products_of<Math, 192, 2, 4, 3>(a, jobs, st);
-    if (kind == TILE_128) return products_of<Math, 128, 2, 4, 4>(a, jobs, st);
-    if (kind == TILE_96) return products_of<Math, 96, 2, 2, 3>(a, jobs, st);
-    if (kind == TILE_64) return products_of<Math, 64, 2, 2, 4>(a, jobs, st);
-    return products_of<Math, 32, 2, 2, 4>(a, jobs, st);
+int products_in(int kind, const NsProducts& a, hipStream_t st) {
+    if (kind == TILE_LARGE) return products_of<Math, 192, 2, 4, 3>(a, st);
+    if (kind == TILE_128) return products_of<Math, 128, 2, 4, 4>(a, st);
+    if (kind == TILE_96) return products_of<Math, 96, 2, 2, 3>(a, st);
+    if (kind == TILE_64) return products_of<Math, 64, 2, 2, 4>(a, st);
+    return products_of<Math, 32, 2, 2, 4>(a, st);
 }
-
-int products(int kind, const NsProducts& a, int jobs, hipStream_t st) { return products_in<MathSplit>(kind, a, jobs, st); }
 
 constexpr int kChainSide = 128;     // A up to this size is worked on by one workgroup
 
@@ -326,7 +342,6 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, float a, float b, flo
     base.l = s.l;
     base.lk = s.lk;
     base.count = s.count;
-    base.tiles = w.square_tiles[0];
     base.slices = 1;
     base.per_slice = lb;
     auto job = [&](const char* P, const char* Q, char* out, float k0, const char* E1, float k1, const char* E2, float k2) {
@@ -350,16 +365,16 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, float a, float b, flo
         const float* factor = (const float*)(ws + w.factor) + (size_t)group * s.count;
         // A = X X'
         NsProducts gram = base;
-        gram.tiles = w.tiles;
         gram.slices = w.slices;
         gram.per_slice = w.per_slice;
         gram.partial = (float*)(ws + w.partial);
         gram.job[0] = job(X, X, A, kScaleA, nullptr, 0.0f, nullptr, 0.0f);
         gram.job[0].factor = factor;
+        gram.job[0].tiles = w.tiles;
         gram.job[0].p_mat = w.x_mat;
         gram.job[0].ldp = w.half ? s.nh * 2 : s.nk * 4;
         gram.job[0].blocks = (int)(gram.job[0].ldp / TILE_BLOCK_BYTES);
-        if (const int rc = w.half ? products_in<MathHalf>(w.gram, gram, 1, st) : products(w.gram, gram, 1, st)) return rc;
+        if (const int rc = w.half ? products_in<MathHalf>(w.gram, gram, st) : products_in<MathSplit>(w.gram, gram, st)) return rc;
         double q = a;                          // Q = q + S
         const char* Q = nullptr;
         float sq = 0.0f;
@@ -381,32 +396,45 @@ int run_steps(const NsShape& s, const Layout& w, char* ws, float a, float b, flo
             for (int j = 1; j < len; ++j) q *= a;
             Q = S[0];
             sq = len == 1 ? kScaleR : kScaleS;
-        } else for (int j = 0; j < len; ++j) {
-            char* Rj = R[j & 1];
-            NsProducts one = base;
-            one.job[0] = job(A, A, Rj, c * kScaleR / (kScaleA * kScaleA), A, b * kScaleR / kScaleA, nullptr, 0.0f);
-            if (const int rc = products(w.square[0], one, 1, st)) return rc;
-            int jobs = 0;
-            NsProducts two = base;
-            const bool last = j + 1 == len;
-            if (!last) two.job[jobs++] = job(Rj, A, T, 1.0f / kScaleR, A, a, nullptr, 0.0f);
-            if (j > 0) {
-                two.job[jobs++] = job(Rj, Q, S[j & 1], kScaleS / (kScaleR * sq), Q, a * kScaleS / sq, Rj, (float)(q * kScaleS / kScaleR));
-                q *= a;
-                Q = S[j & 1];
-                sq = kScaleS;
-            } else {
-                Q = Rj;
-                sq = kScaleR;
-            }
-            if (jobs) {
-                two.tiles = w.square_tiles[jobs - 1];
-                if (const int rc = products(w.square[jobs - 1], two, jobs, st)) return rc;
-            }
-            if (!last) {
-                NsProducts three = base;
-                three.job[0] = job(T, Rj, A, 1.0f / kScaleR, T, a, nullptr, 0.0f);
-                if (const int rc = products(w.square[0], three, 1, st)) return rc;
+        } else {
+            NsProduct waiting = {};            // S of this step, not needed before the next one's
+            int left = 0;
+            auto launch = [&](const NsProduct& p) {
+                NsProducts both = base;
+                both.job[0] = p;
+                both.job[0].tiles = left ? w.shared_tiles : w.square_tiles;
+                if (!left) return products_in<MathSplit>(w.square, both, st);
+                const int64_t share = w.shares - left--;
+                both.job[1] = waiting;
+                both.job[1].first = (int)(w.shared_tiles * share / w.shares);
+                both.job[1].tiles = (int)(w.shared_tiles * (share + 1) / w.shares) - both.job[1].first;
+                return products_in<MathSplit>(w.shared, both, st);
+            };
+            for (int j = 0; j < len; ++j) {
+                char* Rj = j == 0 ? S[0] : R[j & 1];      // S_0 = R_0; neither is written while S of the step before is under way
+                const bool last = j + 1 == len;
+                if (const int rc = launch(job(A, A, Rj, c * kScaleR / (kScaleA * kScaleA), A, b * kScaleR / kScaleA, nullptr, 0.0f))) return rc;
+                NsProduct next = {};
+                if (j > 0) {
+                    next = job(Rj, Q, S[j & 1], kScaleS / (kScaleR * sq), Q, a * kScaleS / sq, Rj, (float)(q * kScaleS / kScaleR));
+                    q *= a;
+                    Q = S[j & 1];
+                    sq = kScaleS;
+                } else {
+                    Q = Rj;
+                    sq = kScaleR;
+                }
+                if (last) {
+                    if (j > 0)
+                        if (const int rc = launch(next)) return rc;
+                    break;
+                }
+                if (j > 0) {
+                    waiting = next;
+                    left = w.shares;
+                }
+                if (const int rc = launch(job(Rj, A, T, 1.0f / kScaleR, A, a, nullptr, 0.0f))) return rc;
+                if (const int rc = launch(job(T, Rj, A, 1.0f / kScaleR, T, a, nullptr, 0.0f))) return rc;
             }
         }
         NsApply ap = {};
