@@ -506,9 +506,9 @@ int yh_linear_i8(const void* x, int x_dtype, int64_t ldx, const float* x_scale, 
  * a matrix taller than wide is worked on transposed, which changes nothing in exact arithmetic.
  * g and out of YH_F32, YH_F16 or YH_BF16; g_stride / out_stride numbers from matrix to matrix, ldg /
  * ldo from row to row, columns next to each other; out must not overlap g or itself.  The matrices are held in
- * 22 bits and summed in fp32: the result is within about 2e-4 of the exact one (relative, whole
- * matrix; YH_F32 results 3e-5) before it is rounded to out_dtype, for coefficients that keep the
- * singular values below 2 (a = 3.4445, b = -4.7750, c = 2.0315 do).  Coefficients and steps under which, with s
+ * 22 bits and summed in fp32: the result is within about 1e-4 of the exact one (relative, whole
+ * matrix of up to a few thousand rows; YH_BF16 results 1e-3) before it is rounded to out_dtype, for
+ * coefficients that keep the singular values below 2 (a = 3.4445, b = -4.7750, c = 2.0315 do).  Coefficients and steps under which, with s
  * in [0, 1] before the first step, s^2, |b s^2 + c s^4| or s^2 |a + b s^2 + c s^4| may pass 120 before a step are
  * refused (YH_ERR_ARG).  Two calls give the same bits.  A NaN or an infinity in a matrix makes all of its
  * result NaN; zeros give zeros.

@@ -17,10 +17,10 @@
 // does what leaks into its direction out of the large ones, so numbers of 8 or 11 bits lose it: against 64 bits,
 // bf16 matrices end 1e-2 to 3e-1 off and fp16 ones 1e-3 to 4e-2 (noise; a few strong directions over noise).
 // Every matrix is therefore held as two fp16 numbers, hi + lo: 22 bits, three matrix-core products for one, fp32
-// sums.  An error of A grows by a^2 a step, which limits how many steps one A may serve: five end 1e-5 to 2e-4 off,
-// three and two with a fresh A in between 3e-6 to 3e-5, an A for every step 2e-6 to 2e-5 -- the last is what fp32
-// arithmetic gives.  The entry points form a new A when a^steps would pass 64 (fp32 results) or 511 (16-bit
-// results, whose own rounding is 2e-3).
+// sums.  An error of A grows by a^2 a step, which limits how many steps one A may serve: measured over 16 x 16 to
+// 4096 x 9216 and spectra from noise to one strong direction over 1 % of it, five end 6e-6 to 8e-4 off, three and two
+// with a fresh A in between 2e-6 to 5.5e-5, where fp32 arithmetic with an A for every step ends 7e-7 to 7.4e-5 off.
+// The entry points form a new A when a^steps would pass 64, or 511 for bf16 results, whose own rounding is 1.7e-3.
 //
 // X is held as a matrix of Frobenius norm `scale` and the factor |G| / (|G| + eps) / scale beside it, a number of its own for
 // each matrix: a gradient far below eps keeps its bits.  What is held grows with the steps, by `growth` as long as the singular

@@ -275,7 +275,8 @@ int load_as(int dt, const NsSource& src, const NsShape& s, const Layout& w, char
 
 // The steps in groups, each on one X X'.  A singular value s of X becomes s (a + b s^2 + c s^4): from all of [0, 1] that gives
 // the largest one before every step, and the largest factor of every step.  A group ends where the product of its factors
-// would pass 64 (fp32 results) or 511 (16-bit results, S within its range).
+// would pass 64, or 511 for bf16 results (S within its range): the error of one X X' for five steps, 8e-4 at most, is
+// below bf16's own rounding (1.7e-3) but not fp16's (2.1e-4).
 struct Steps {
     NsHold hold;
     int len[NS_MAX_GROUPS];
@@ -287,7 +288,7 @@ inline short above(double x) { return (short)(x > 1e-30 ? ilogb(x) + 1 : -99); }
 
 // false: coefficients and steps whose matrices would leave fp16's range
 bool steps_in_groups(double a, double b, double c, int steps, int out_dtype, double scale, Steps& p) {
-    const double limit = out_dtype == YH_F32 ? 64.0 : 511.0;
+    const double limit = out_dtype == YH_BF16 ? 511.0 : 64.0;
     double top = 1.0, growth = 1.0, within = 1.0;
     bool full = true;
     p.hold.groups = 0;
@@ -325,7 +326,7 @@ bool steps_in_groups(double a, double b, double c, int steps, int out_dtype, dou
 }
 
 // X in fp16 alone: 16-bit numbers, all steps on one X X', and enough of them to pay for the launch that lays S out in
-// planes (a call in us, split / half: 192x576 85.6 / 90.1, 512x512 113 / 117, 256x4096 104.5 / 102.3, 512x2304 129 / 127,
+// planes (a call in us with bf16 results, split / half: 192x576 85.6 / 90.1, 512x512 113 / 117, 256x4096 104.5 / 102.3, 512x2304 129 / 127,
 // 4x512x2304 202 / 195, 1470x4096 475 / 443, 4x1024x9216 897 / 740, 4096x50,176 9520 / 7210)
 bool half_for(const NsShape& s, int g_dtype, int out_dtype, const Steps& plan) {
     return g_dtype != YH_F32 && out_dtype != YH_F32 && s.l > 128 && plan.hold.groups == 1 &&
