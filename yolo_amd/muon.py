@@ -160,14 +160,27 @@ class Muon(torch.optim.Optimizer):
                     raise ValueError(f"Muon: a parameter of shape {tuple(p.shape)}; weights of two or more axes only")
 
     def load_state_dict(self, state_dict):
-        super().load_state_dict(state_dict)
-        # torch has cast the momenta to the types of their weights
-        keys = [key for group in state_dict["param_groups"] for key in group["params"]]
-        weights = [p for group in self.param_groups for p in group["params"]]
-        for key, p in zip(keys, weights):
-            saved = state_dict["state"].get(key, {}).get("momentum_buffer")
-            if saved is not None:
-                self.state[p]["momentum_buffer"] = saved.detach().to(p.device, torch.float32, copy=True).contiguous()
+        # torch casts a loaded state to the types of its weights; momenta stay fp32.  They come from what the last
+        # pre-hook leaves, and the first post-hook finds them in place.
+        loaded = {}
+
+        def keep(_, given):
+            loaded.update(given)
+
+        def restore(_):
+            keys = [key for group in loaded["param_groups"] for key in group["params"]]
+            weights = [p for group in self.param_groups for p in group["params"]]
+            for key, p in zip(keys, weights):
+                saved = loaded["state"].get(key, {}).get("momentum_buffer")
+                if saved is not None:
+                    self.state[p]["momentum_buffer"] = saved.detach().to(p.device, torch.float32, copy=True).contiguous()
+
+        hooks = [self.register_load_state_dict_pre_hook(keep), self.register_load_state_dict_post_hook(restore, prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
 
     @torch.no_grad()
     def step(self, closure=None):
