@@ -5,6 +5,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -36,6 +37,25 @@ class _on_device:
         if self.ctx is not None:
             self.ctx.__exit__(*exc)
         return False
+
+
+def _tensor(t, name: str, op: str) -> torch.Tensor:
+    """A tensor without a forward-mode tangent, which ``op`` would drop."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
+    # the level is -1 outside of forward mode, and asking every tensor costs 0.5 us each
+    if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name}: carries a tangent, and {op} has none; pass its primal part")
+    return t
+
+
+def _forward_only(t, name: str, op: str) -> torch.Tensor:
+    """A tensor of which neither a gradient nor a tangent is asked for: ``op`` has none, and would drop it."""
+    _tensor(t, name, op)
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name}: requires a gradient, and {op} has none; call it under torch.no_grad() or on a "
+                         "detached tensor")
+    return t
 
 
 def _need(t: torch.Tensor, name: str, dtype, shape=None) -> torch.Tensor:

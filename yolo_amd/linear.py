@@ -5,7 +5,8 @@ the input (an image's features) and of the weight (an output channel).
     layer = Int8Linear.from_linear(net[-1])               # weights quantised and laid out once
     dets, count = head.postprocess_linear(features, layer)
 
-The sum is exact in int32; scales and bias are applied in fp32.  Forward only."""
+The sum is exact in int32; scales and bias are applied in fp32.  Forward only: an input, scale or bias that
+requires a gradient while gradients are recorded is refused."""
 from __future__ import annotations
 
 from functools import lru_cache
@@ -15,7 +16,7 @@ import torch
 from torch import nn
 
 from . import _lib
-from ._tensors import _need, _on_device, _ptr, _stream
+from ._tensors import _forward_only, _need, _on_device, _ptr, _stream
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
@@ -25,16 +26,8 @@ def _workspace_bytes(code: int, m: int, n: int, k: int) -> int:
     return _lib.load().yh_linear_i8_workspace_bytes(code, m, n, k)
 
 
-def _no_grad(t: torch.Tensor, name: str) -> None:
-    if torch.is_grad_enabled() and t.requires_grad:
-        raise ValueError(f"{name}: requires a gradient, and the 8-bit product has none; call it under "
-                         "torch.no_grad() or on a detached tensor")
-
-
 def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
     """(..., K) as (M, K) with unit stride along K; a view where the strides allow one."""
-    if not isinstance(x, torch.Tensor):
-        raise TypeError(f"{name}: expected a torch.Tensor, got {type(x).__name__}")
     if not x.is_cuda:
         raise ValueError(f"{name}: must live on the GPU (got device {x.device}); yolo_amd has no CPU path")
     if x.dim() < 1 or not 1 <= x.shape[-1] <= _lib.YH_MAX_I8_K:
@@ -61,8 +54,8 @@ def quantize_rows(x: torch.Tensor):
     ``q`` has shape (M, K); its rows lie a multiple of 128 bytes apart with zeros behind them, the
     layout ``linear_i8`` takes for a weight.  A row of zeros gets scale 0; a row that holds a NaN or
     an infinity gets scale NaN and zeros."""
-    _no_grad(x, "x")
-    if isinstance(x, torch.Tensor) and x.dim() != 2:
+    _forward_only(x, "x", "quantize_rows")
+    if x.dim() != 2:
         raise ValueError(f"x: expected shape (M, K), got {tuple(x.shape)}")
     x = _rows(x, "x")
     if x.dtype not in _FLOATS:
@@ -84,7 +77,9 @@ def linear_i8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
     scales of its rows in ``x_scale``.  ``weight`` as ``quantize_rows`` returns it: unit stride along K, rows a
     multiple of 16 bytes apart.  ``bias`` (N) fp32.  The result has ``out_dtype`` (fp32, fp16, bf16; by
     default that of ``x``, fp32 for an int8 ``x``)."""
-    _no_grad(x, "x")
+    for name, t in (("x", x), ("weight_scale", weight_scale), ("bias", bias), ("x_scale", x_scale)):
+        if t is not None or name in ("x", "weight_scale"):
+            _forward_only(t, name, "linear_i8")
     shape = x.shape
     x = _rows(x, "x")
     m, k = x.shape

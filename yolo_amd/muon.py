@@ -16,7 +16,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from ._tensors import _need, _on_device, _stream
+from ._tensors import _forward_only, _need, _on_device, _stream, _tensor
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 COEFFS = (3.4445, -4.7750, 2.0315)      # raises small singular values fastest; they end within 0.7 .. 1.2
@@ -58,14 +58,11 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coeffs: Tuple[float, float, f
     The matrices are held in 22 bits: the result (contiguous, ``out_dtype``) is within about 1e-4 of the exact
     one (whole matrix, relative; 1e-3 when it is bf16) before its rounding, for matrices of up to a few thousand rows.  Coefficients and steps under which singular values would grow
     out of range (past 10) are refused.  A NaN or an infinity makes its whole matrix NaN.  Forward only."""
-    if not isinstance(g, torch.Tensor):
-        raise TypeError(f"g: expected a torch.Tensor, got {type(g).__name__}")
+    _forward_only(g, "g", "orthogonalize")
     if not g.is_cuda:
         raise ValueError(f"g: must live on the GPU (got device {g.device}); yolo_amd has no CPU path")
     if g.dtype not in _FLOATS or out_dtype not in _FLOATS:
         raise ValueError(f"g and out_dtype: expected float32, float16 or bfloat16, got {g.dtype} and {out_dtype}")
-    if torch.is_grad_enabled() and g.requires_grad:
-        raise ValueError("g: requires a gradient, and orthogonalize has none; pass g.detach()")
     if g.dim() < 2:
         raise ValueError(f"g: expected shape (..., rows, cols), got {tuple(g.shape)}")
     _check_steps(steps, eps)
@@ -98,11 +95,14 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
     ``params`` (fp32, fp16 or bf16), ``grads`` (fp32, fp16 or bf16) and ``momenta`` (fp32) are sequences of
     contiguous tensors of one shape each; an axis beyond the second is folded into the columns (a
     convolution's cout x cin*k*k).  ``scale`` defaults to ``sqrt(max(1, rows / cols))``.  A captured graph replays
-    the step with the tensors and numbers it was captured with."""
+    the step with the tensors and numbers it was captured with.  Autograd does not record the step."""
     if not (len(params) == len(grads) == len(momenta)):
         raise ValueError(f"{len(params)} params, {len(grads)} grads and {len(momenta)} momenta")
     if not params:
         return
+    for name, tensors in (("params", params), ("grads", grads), ("momenta", momenta)):
+        for i, t in enumerate(tensors):
+            _tensor(t, f"{name}[{i}]", "muon_step")
     first = params[0]
     shape, dev = tuple(first.shape), first.device
     if len(shape) < 2:
