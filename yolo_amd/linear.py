@@ -127,7 +127,8 @@ def linear_i8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
 
 class Int8Linear(nn.Module):
     """A linear layer served in 8-bit integers: ``forward(x)`` is ``linear_i8`` with this layer's weight,
-    scales and bias.  The weight is quantised and laid out once, by ``from_linear``."""
+    scales and bias.  The weight is quantised and laid out once, by ``from_linear``; weight, scales and bias keep
+    their types when the network around them is moved to another (``half()``, ``to(dtype)``)."""
 
     def __init__(self, weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optional[torch.Tensor] = None):
         super().__init__()
@@ -137,6 +138,16 @@ class Int8Linear(nn.Module):
         self.register_buffer("weight_rows", rows)
         self.register_buffer("weight_scale", weight_scale.detach().clone())
         self.register_buffer("bias", None if bias is None else bias.detach().float().clone())
+
+    def _apply(self, fn, recurse=True):
+        # A network moved to another number type takes the layer along, but the layer keeps its own types: integers for the
+        # weight, fp32 for scales and bias.
+        held = dict(self._buffers)
+        super()._apply(fn, recurse)
+        for name, old in held.items():
+            if old is not None and self._buffers[name].dtype != old.dtype:
+                self._buffers[name] = old.to(self._buffers[name].device)
+        return self
 
     @classmethod
     def from_linear(cls, linear: nn.Linear) -> "Int8Linear":
