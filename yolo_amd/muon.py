@@ -146,8 +146,9 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
 
 
 class Muon(torch.optim.Optimizer):
-    """``muon_step`` as an optimizer over weights of two or more axes (convolutions, linear layers); biases and
-    norms belong to another optimizer.  Weights of one shape and type are stepped together."""
+    """``muon_step`` as an optimizer over weights of two or more axes (convolutions, linear layers), contiguous or
+    channels-last; biases and norms belong to another optimizer.  Weights of one shape, type and layout are stepped together.
+    The types and layouts of all weights are looked at before any is changed."""
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, weight_decay: float = 0.0, nesterov: bool = True,
                  steps: int = 5, coeffs: Tuple[float, float, float] = COEFFS, eps: float = 1e-7):
@@ -173,7 +174,7 @@ class Muon(torch.optim.Optimizer):
             for key, p in zip(keys, weights):
                 saved = loaded["state"].get(key, {}).get("momentum_buffer")
                 if saved is not None:
-                    self.state[p]["momentum_buffer"] = saved.detach().to(p.device, torch.float32, copy=True).contiguous()
+                    self.state[p]["momentum_buffer"] = torch.empty_like(p, dtype=torch.float32, requires_grad=False).copy_(saved.detach())
 
         hooks = [self.register_load_state_dict_pre_hook(keep), self.register_load_state_dict_post_hook(restore, prepend=True)]
         try:
@@ -188,21 +189,60 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        for group in self.param_groups:
+        groups, unmade = [], set()
+        for group in self.param_groups:               # all of them are looked at before anything is made or changed
             alike = {}
             for p in group["params"]:
                 if p.grad is None:
                     continue
-                state = self.state[p]
-                if "momentum_buffer" not in state:
-                    if torch.cuda.is_current_stream_capturing():
-                        raise RuntimeError("Muon: the first step of a weight makes its momentum, and a captured graph would clear it "
-                                           "in every replay; take one step before the capture")
-                    state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
-                alike.setdefault((tuple(p.shape), p.dtype, p.grad.dtype, p.device), []).append(p)
-            for ps in alike.values():
-                muon_step(ps, [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p in ps],
-                          [self.state[p]["momentum_buffer"] for p in ps], lr=group["lr"], momentum=group["momentum"],
+                if p.dim() < 2:
+                    raise ValueError(f"Muon: a parameter of shape {tuple(p.shape)}; weights of two or more axes only")
+                if p.dtype not in _FLOATS or p.grad.dtype not in _FLOATS or p.grad.layout != torch.strided:
+                    raise ValueError("Muon: expected weights and dense gradients of float32, float16 or bfloat16, got "
+                                     f"{p.dtype} and {p.grad.dtype}, {p.grad.layout}")
+                order = _rows_outermost(p)
+                held = self.state[p].get("momentum_buffer") if p in self.state else None
+                if held is None or not _in_order(held, order).is_contiguous():
+                    unmade.add(p.device)
+                alike.setdefault((tuple(p.shape), p.dtype, p.grad.dtype, p.device, order), []).append(p)
+            groups.append((group, alike))
+        for dev in unmade:
+            with _on_device(dev):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("Muon: the first step of a weight, or of one that was laid out anew, makes its momentum, and a "
+                                       "captured graph would make it in every replay; take one step before the capture")
+            if dev.type != "cuda":
+                raise ValueError(f"Muon: a parameter on {dev}; yolo_amd has no CPU path")
+        for group, alike in groups:
+            for (*_, order), ps in alike.items():
+                momenta = [self._momentum(p, order) for p in ps]
+                muon_step([_in_order(p, order) for p in ps], [_in_order(p.grad, order).contiguous() for p in ps],
+                          [_in_order(m, order) for m in momenta], lr=group["lr"], momentum=group["momentum"],
                           weight_decay=group["weight_decay"], nesterov=group["nesterov"], steps=group["steps"],
                           coeffs=group["coeffs"], eps=group["eps"])
         return loss
+
+    def _momentum(self, p: torch.Tensor, order) -> torch.Tensor:
+        """The momentum of ``p``, lying as ``p`` does."""
+        state = self.state[p]
+        held = state.get("momentum_buffer")
+        if held is None or not _in_order(held, order).is_contiguous():
+            new = torch.zeros_like(p, dtype=torch.float32, requires_grad=False)
+            state["momentum_buffer"] = new if held is None else new.copy_(held)
+        return state["momentum_buffer"]
+
+
+def _rows_outermost(p: torch.Tensor) -> Optional[Tuple[int, ...]]:
+    """The order of axes, the first one staying first, in which ``p`` is contiguous (None: as they are).  A channels-last
+    convolution is a matrix whose columns come in another order, and so do those of its update."""
+    if p.is_contiguous():
+        return None
+    order = (0, *sorted(range(1, p.dim()), key=p.stride, reverse=True))
+    if not p.permute(order).is_contiguous():
+        raise ValueError(f"Muon: a parameter of shape {tuple(p.shape)} and strides {p.stride()}; its numbers must lie next to each "
+                         "other with the first axis outermost (contiguous or channels-last)")
+    return order
+
+
+def _in_order(t: torch.Tensor, order: Optional[Tuple[int, ...]]) -> torch.Tensor:
+    return t if order is None else t.permute(order)
