@@ -67,6 +67,7 @@ extern "C" {
 #define YH_I8 3
 
 #define YH_MAX_I8_K 131071   /* yh_linear_i8: 128 * 128 * K stays below 2^31 */
+#define YH_MAX_I8_ROWS 4194303 /* yh_quantize_rows, yh_linear_i8: rows, M and N */
 #define YH_MAX_NS_STEPS 64   /* yh_orthogonalize, yh_muon_step */
 #define YH_MUON_MAX_COUNT 32 /* matrices of one yh_muon_step call */
 
@@ -488,6 +489,7 @@ int yh_nms_ws(const float* cand_ltrb, const float* cand_score, const int32_t* ca
  * With YH_F32 and no bias y is the z of yh_decode_nms_linear.
  * workspace: yh_linear_i8_workspace_bytes bytes, 256-byte aligned, contents never matter (NULL where
  * it answers 0: a few rows are quantised on the way).
+ * Limits: rows, M and N <= YH_MAX_I8_ROWS, K <= YH_MAX_I8_K, and y of fewer than 2^24 tiles of 32 x 32.
  */
 int yh_quantize_rows(const void* x, int x_dtype, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
                      int64_t rows, int64_t K, void* stream);
@@ -520,7 +522,8 @@ int yh_linear_i8(const void* x, int x_dtype, int64_t ldx, const float* x_scale, 
  * and numbers are what a captured graph replays.  No two params or momenta may overlap.
  *
  * workspace (both): yh_orthogonalize_workspace_bytes bytes, 256-byte aligned, contents never
- * matter.  Limits: the shorter side <= 32,768, the longer <= 2^24, steps <= YH_MAX_NS_STEPS.
+ * matter; it serves every type and number of steps.  Limits: the shorter side <= 32,768, the longer <= 2^24, count <= 65,535,
+ * count * ceil(rows / 32) * ceil(cols / 32) < 2^24, steps <= YH_MAX_NS_STEPS.
  */
 size_t yh_orthogonalize_workspace_bytes(int64_t count, int64_t rows, int64_t cols);
 int yh_orthogonalize(const void* g, int g_dtype, int64_t g_stride, int64_t ldg, void* out,

@@ -43,6 +43,7 @@ YH_I8 = 3
 DTYPE_CODES = {torch.float32: YH_F32, torch.float16: YH_F16, torch.bfloat16: YH_BF16, torch.int8: YH_I8}
 
 YH_MAX_I8_K = 131071
+YH_MAX_I8_ROWS = 4194303
 YH_MAX_NS_STEPS = 64
 YH_MUON_MAX_COUNT = 32
 

@@ -18,7 +18,7 @@ inline int launch_status() {
 }
 inline size_t dtype_bytes(int dt) { return dt == YH_F32 ? 4 : dt == YH_I8 ? 1 : 2; }
 
-constexpr int64_t kMaxRows = ((int64_t)1 << 22) - 1;      // a grid holds fewer than 2^32 threads, a row takes up to 1,024
+constexpr int64_t kMaxRows = YH_MAX_I8_ROWS;      // a grid holds fewer than 2^32 threads, a row takes up to 1,024
 
 // tops: rows * QUANT_PARTS words for the shared form, or null (yh_quantize_rows has no workspace)
 template <int DT>

@@ -34,6 +34,8 @@ def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
         raise ValueError(f"{name}: expected shape (..., K) with K in 1 .. {_lib.YH_MAX_I8_K}, got {tuple(x.shape)}")
     if x.stride(-1) != 1 and x.shape[-1] > 1:
         raise ValueError(f"{name}: must be contiguous along its last axis")
+    if x.numel() // x.shape[-1] > _lib.YH_MAX_I8_ROWS:
+        raise ValueError(f"{name}: expected at most {_lib.YH_MAX_I8_ROWS:,} rows, got shape {tuple(x.shape)}")
     if x.requires_grad:
         x = x.detach()
     if x.dim() != 2:
@@ -96,6 +98,9 @@ def linear_i8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.shape[1] != k or weight.dtype != torch.int8:
         raise ValueError(f"weight: expected an int8 tensor of shape (N, {k})")
     n = weight.shape[0]
+    if n > _lib.YH_MAX_I8_ROWS or ((m + 31) // 32) * ((n + 31) // 32) >= 1 << 24:
+        raise ValueError(f"weight: expected at most {_lib.YH_MAX_I8_ROWS:,} rows, and a result of fewer than 2^24 tiles of 32 x 32; got "
+                         f"{m} x {n}")
     room = (k + 15) // 16 * 16
     ldw, along = weight.stride()
     ldw = ldw if n > 1 else room

@@ -30,22 +30,33 @@ def _workspace_bytes(count: int, rows: int, cols: int) -> int:
 def _workspace(count: int, rows: int, cols: int, device) -> torch.Tensor:
     nbytes = _workspace_bytes(count, rows, cols)
     if nbytes == 0:
-        raise ValueError(f"{count} matrices of {rows} x {cols}: outside the supported range (shorter side up to 32,768, "
-                         "longer up to 2^24)")
+        raise ValueError(f"{count} matrices of {rows} x {cols}: outside the supported range (at most 65,535 matrices, shorter side "
+                         "up to 32,768, longer up to 2^24, and in all fewer than 2^24 tiles of 32 x 32)")
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+_MOST = 3.4028234663852886e38       # of fp32
 
 
 def _check_steps(steps: int, eps: float) -> None:
     if not 1 <= int(steps) <= _lib.YH_MAX_NS_STEPS:
         raise ValueError(f"steps: expected 1 .. {_lib.YH_MAX_NS_STEPS}, got {steps}")
-    if not (eps >= 0 and math.isfinite(eps)):
+    if not 0 <= eps <= _MOST:
         raise ValueError(f"eps: expected a finite number that is not negative, got {eps}")
+
+
+def _check_numbers(coeffs, **numbers) -> None:
+    if len(coeffs) != 3:
+        raise ValueError(f"coeffs: expected three numbers, got {len(coeffs)}")
+    for name, value in (*numbers.items(), *((f"coeffs[{i}]", v) for i, v in enumerate(coeffs))):
+        if not abs(value) <= _MOST:
+            raise _lib.YoloHeadError(_lib.YH_ERR_ARG, f"{name}: expected a finite number (in fp32), got {value}")
 
 
 def _check(rc: int) -> None:
     if rc == _lib.YH_ERR_ARG:
-        raise _lib.YoloHeadError(rc, "coeffs: coefficients under which so many steps leave the supported range (singular values "
-                                     "past 10), or a number that is not finite")
+        raise _lib.YoloHeadError(rc, "coeffs: coefficients under which so many steps leave the supported range: with singular "
+                                     "values s in [0, 1], s^2, |b s^2 + c s^4| or s^2 |a + b s^2 + c s^4| may pass 120 before a step")
     _lib.check(rc)
 
 
@@ -56,16 +67,17 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coeffs: Tuple[float, float, f
 
     Columns lie next to each other and rows at any stride of at least ``cols``; leading axes collapse to one.
     The matrices are held in 22 bits: the result (contiguous, ``out_dtype``) is within about 1e-4 of the exact
-    one (whole matrix, relative; 1e-3 when it is bf16) before its rounding, for matrices of up to a few thousand rows.  Coefficients and steps under which singular values would grow
-    out of range (past 10) are refused.  A NaN or an infinity makes its whole matrix NaN.  Forward only."""
+    one (whole matrix, relative; 1e-3 when it is bf16) before its rounding, for matrices of up to a few thousand rows.  Coefficients and steps under which, with singular
+    values s in [0, 1], s^2, |b s^2 + c s^4| or s^2 |a + b s^2 + c s^4| may pass 120 before a step are refused.  A NaN or an infinity makes its whole matrix NaN.  Forward only."""
     _forward_only(g, "g", "orthogonalize")
+    _check_steps(steps, eps)
+    _check_numbers(coeffs)
     if not g.is_cuda:
         raise ValueError(f"g: must live on the GPU (got device {g.device}); yolo_amd has no CPU path")
     if g.dtype not in _FLOATS or out_dtype not in _FLOATS:
         raise ValueError(f"g and out_dtype: expected float32, float16 or bfloat16, got {g.dtype} and {out_dtype}")
     if g.dim() < 2:
         raise ValueError(f"g: expected shape (..., rows, cols), got {tuple(g.shape)}")
-    _check_steps(steps, eps)
     out = torch.empty(g.shape, dtype=out_dtype, device=g.device)
     if g.numel() == 0:
         return out
@@ -103,6 +115,8 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
     for name, tensors in (("params", params), ("grads", grads), ("momenta", momenta)):
         for i, t in enumerate(tensors):
             _tensor(t, f"{name}[{i}]", "muon_step")
+    _check_steps(steps, eps)
+    _check_numbers(coeffs, lr=lr, momentum=momentum, weight_decay=weight_decay, scale=0.0 if scale is None else scale)
     first = params[0]
     shape, dev = tuple(first.shape), first.device
     if len(shape) < 2:
@@ -115,7 +129,6 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
             _need(t.detach(), f"{name}[{i}]", dtype, shape)
             if t.device != dev:
                 raise ValueError(f"{name}[{i}]: on {t.device}, params[0] is on {dev}")
-    _check_steps(steps, eps)
     if first.numel() == 0:
         return
     spans = sorted([(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), 1) for t in (*params, *momenta)]
