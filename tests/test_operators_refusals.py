@@ -71,3 +71,11 @@ def test_refused_sizes_and_coefficients_state_their_limits(dev):
     a, b = torch.zeros(1 << 17, 16, dtype=torch.int8, device=dev), torch.zeros(1 << 17, device=dev)
     with pytest.raises(ValueError, match="tiles"):
         linear_i8(a, a, b, x_scale=b, out_dtype=torch.float16)
+
+
+@pytest.mark.gpu
+def test_a_weight_elsewhere_is_named(dev):
+    x = torch.ones(4, 16, device=dev)
+    w, t = quantize_rows(torch.ones(3, 16, device=dev))
+    with pytest.raises(ValueError, match=r"weight: on cpu, x is on cuda:0"):
+        linear_i8(x, torch.zeros(3, 16, dtype=torch.int8), t)

@@ -16,7 +16,7 @@ import torch
 from torch import nn
 
 from . import _lib
-from ._tensors import _forward_only, _need, _on_device, _ptr, _stream
+from ._tensors import _forward_only, _need, _on_device, _plain, _ptr, _stream
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
@@ -30,17 +30,20 @@ def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
     """(..., K) as (M, K) with unit stride along K; a view where the strides allow one."""
     if not x.is_cuda:
         raise ValueError(f"{name}: must live on the GPU (got device {x.device}); yolo_amd has no CPU path")
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= _lib.YH_MAX_I8_K:
-        raise ValueError(f"{name}: expected shape (..., K) with K in 1 .. {_lib.YH_MAX_I8_K}, got {tuple(x.shape)}")
-    if x.stride(-1) != 1 and x.shape[-1] > 1:
+    shape = x.shape
+    if not shape or not 1 <= shape[-1] <= _lib.YH_MAX_I8_K:
+        raise ValueError(f"{name}: expected shape (..., K) with K in 1 .. {_lib.YH_MAX_I8_K}, got {tuple(shape)}")
+    k = shape[-1]
+    if k > 1 and x.stride(-1) != 1:
         raise ValueError(f"{name}: must be contiguous along its last axis")
-    if x.numel() // x.shape[-1] > _lib.YH_MAX_I8_ROWS:
-        raise ValueError(f"{name}: expected at most {_lib.YH_MAX_I8_ROWS:,} rows, got shape {tuple(x.shape)}")
+    m = shape[0] if len(shape) == 2 else x.numel() // k
+    if m > _lib.YH_MAX_I8_ROWS:
+        raise ValueError(f"{name}: expected at most {_lib.YH_MAX_I8_ROWS:,} rows, got shape {tuple(shape)}")
     if x.requires_grad:
         x = x.detach()
-    if x.dim() != 2:
-        x = x.reshape(-1, x.shape[-1]) if x.numel() else x.new_empty(0, x.shape[-1])
-    if x.shape[0] > 1 and x.stride(0) < x.shape[1]:      # expanded or overlapping rows
+    if len(shape) != 2:
+        x = x.reshape(-1, k) if m else x.new_empty(0, k)
+    if m > 1 and x.stride(0) < k:                        # expanded or overlapping rows
         x = x.contiguous()
     return x
 
@@ -79,9 +82,10 @@ def linear_i8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
     scales of its rows in ``x_scale``.  ``weight`` as ``quantize_rows`` returns it: unit stride along K, rows a
     multiple of 16 bytes apart.  ``bias`` (N) fp32.  The result has ``out_dtype`` (fp32, fp16, bf16; by
     default that of ``x``, fp32 for an int8 ``x``)."""
-    for name, t in (("x", x), ("weight_scale", weight_scale), ("bias", bias), ("x_scale", x_scale)):
-        if t is not None or name in ("x", "weight_scale"):
-            _forward_only(t, name, "linear_i8")
+    if x is None or not _plain(x, weight_scale, bias, x_scale):
+        for name, t in (("x", x), ("weight_scale", weight_scale), ("bias", bias), ("x_scale", x_scale)):
+            if t is not None or name == "x":
+                _forward_only(t, name, "linear_i8")
     shape = x.shape
     x = _rows(x, "x")
     m, k = x.shape
@@ -98,7 +102,7 @@ def linear_i8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.shape[1] != k or weight.dtype != torch.int8:
         raise ValueError(f"weight: expected an int8 tensor of shape (N, {k})")
     n = weight.shape[0]
-    if n > _lib.YH_MAX_I8_ROWS or ((m + 31) // 32) * ((n + 31) // 32) >= 1 << 24:
+    if n > _lib.YH_MAX_I8_ROWS or (m + 31) // 32 * ((n + 31) // 32) >= 1 << 24:
         raise ValueError(f"weight: expected at most {_lib.YH_MAX_I8_ROWS:,} rows, and a result of fewer than 2^24 tiles of 32 x 32; got "
                          f"{m} x {n}")
     room = (k + 15) // 16 * 16
@@ -111,9 +115,11 @@ def linear_i8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
     _need(weight_scale, "weight_scale", torch.float32, (n,))
     if bias is not None:
         _need(bias, "bias", torch.float32, (n,))
-    for name, t in (("weight", weight), ("weight_scale", weight_scale), ("bias", bias), ("x_scale", x_scale)):
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name}: on {t.device}, x is on {dev}")
+    if (weight.device != dev or weight_scale.device != dev or (bias is not None and bias.device != dev)
+            or (x_scale is not None and x_scale.device != dev)):
+        places = {name: t.device for name, t in (("weight", weight), ("weight_scale", weight_scale), ("bias", bias),
+                                                 ("x_scale", x_scale)) if t is not None and t.device != dev}
+        raise ValueError(f"{', '.join(places)}: on {', '.join(map(str, places.values()))}, x is on {dev}")
     if out_dtype is None:
         out_dtype = torch.float32 if code == _lib.YH_I8 else x.dtype
     if out_dtype not in _FLOATS:
