@@ -75,8 +75,9 @@ __device__ __forceinline__ int quantize_one(float x, double inv) {
 __device__ __forceinline__ unsigned magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
 // N numbers: x * inv in fp32 is off by at most 127 * 2^-23, so its nearest whole number is the right one unless it lies
-// that close to the middle of two; then (one group of 16 in a thousand, and where numbers are halves of the
-// largest) the group is done again in 64 bits.  Three times fewer cycles than 64 bits throughout.
+// that close to the middle of two; then (one number in 5,000, three groups of 16 in a thousand, and where numbers are halves of
+// the largest) the group is done again in 64 bits, by the whole wavefront: one of its passes in five.  A pass without it
+// takes a third of the cycles of 64 bits throughout, so the mean is about half.
 template <int N>
 __device__ __forceinline__ void quantize_some(const float (&x)[N], double inv, int8_t (&q)[N]) {
     const float f = (float)inv;
@@ -147,8 +148,8 @@ union Quantized {
 
 // One workgroup per row, a thread 16 numbers at a time, held in registers between the maximum and the division
 // (K <= THREADS * 16 * CHUNKS): every byte is read once and a row costs one trip to memory.  Zeros are written from K to
-// Kz, a multiple of 16: the padding the product's blocks of 128 bytes read.  8,192 rows of 4,096 bf16: 21 to 25 us,
-// 4.0 to 4.8 TB/s; 4,096 rows of 4,096 fp32: 15 us, 5.5 TB/s.
+// Kz, a multiple of 16: the padding the product's blocks of 128 bytes read.  8,192 rows of 4,096 bf16: 23 to 28 us,
+// 3.6 to 4.3 TB/s; 4,096 rows of 4,096 fp32: 15 us, 5.5 TB/s.
 template <int DT, int THREADS, int CHUNKS>
 __global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const typename Elem<DT>::T* __restrict__ x, long long ldx,
                                                                 int8_t* __restrict__ q, long long ldq,
@@ -177,7 +178,7 @@ __global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const typename E
 }
 
 // Few long rows: a CU alone takes 4 us to bring in 100 KB, so PARTS workgroups share a row in two launches, the largest
-// magnitudes of the parts first (tops: rows x PARTS).  64 rows of 50,176: 4.6 + 4.6 instead of
+// magnitudes of the parts first (tops: rows x PARTS).  64 rows of 50,176: 4.4 to 4.8 us each instead of
 // 11 us.
 constexpr int QUANT_PARTS = 16;
 
@@ -409,7 +410,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_i8_tile_kernel(LinearI
 // blocks (8 KB) on their way while four are worked on; the 16 sums meet in LDS.  STAGE: every workgroup brings the rows of x
 // into LDS for itself, quantised where they are not 8-bit already and padded with zeros, while its first weights are on
 // their way: for few rows that is less than a launch of its own.  Otherwise a.q holds the padded rows.  1 x 4096 -> 1470:
-// 6 us (6.0 MB; the host's part of a call is 11); 1 x 50,176 -> 4096: 45 us, 4.6 TB/s of weights (copies reach 5.1).  Loads past the end of
+// 7 us (6.0 MB; the host's part of a call is 11); 1 x 50,176 -> 4096: 44 to 46 us, 4.5 to 4.7 TB/s of weights (copies reach 5.1).  Loads past the end of
 // a row, the same line from every wavefront, took 1 x 4096 to 13 us: none is issued.
 template <int DTX, int DT, bool STAGE>
 __global__ __launch_bounds__(1024) void linear_i8_rows_kernel(LinearI8Args a, const typename Elem<DTX>::T* __restrict__ x,

@@ -115,9 +115,10 @@ Plan plan_for(int64_t M, int64_t N, int64_t K) {
 }
 
 constexpr int kRows = 16;      // rows of a workgroup of linear_i8_rows_kernel
-// It brings the rows into LDS itself when that is less than a launch by itself (us, with / without: 1 x 4096 5.7 / 7.1, 4 x 4096
-// 8.0 / 7.8, 16 x 4096 14.2 / 8.9, 1 x 50,176 46.1 / 50.5): up to 12,288 numbers or one row (8-bit rows, which are only
-// copied: 65,536 bytes), and one workgroup a CU (64 x 700 -> 1470, 368 workgroups: 19.8 / 8.1).
+// It brings the rows into LDS itself when that is less than a launch by itself (bf16 rows, kernel times in us of calls on one
+// weight, with / without, the latter both launches: 1 x 4096 -> 1470 6.8 / 7.6, 4 x 4096 7.8 / 8.3, 16 x 4096 14.0 / 9.6, 1 x
+// 50,176 -> 4096 39.2 / 43.7): up to 12,288 numbers or one row (8-bit rows, which are only copied: 65,536 bytes), and one
+// workgroup a CU (64 x 700 -> 1470, 368 workgroups: 19.7 / 7.9).
 inline bool stages_itself(int x_dtype, int64_t M, int64_t N, int64_t blocks) {
     const int64_t rows = M < kRows ? M : kRows;
     if (((M + kRows - 1) / kRows) * ((N + 15) / 16) > 256) return M <= kRows && M * blocks <= 96;

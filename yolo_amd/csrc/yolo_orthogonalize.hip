@@ -25,6 +25,7 @@ constexpr int64_t kMaxShort = 32768, kMaxLong = (int64_t)1 << 24, kMaxNumbers = 
 // 4.4, 512 (4) 31 / 15 / 17.7 / 8.9 / 8.6, 1024 44 / 22 / 23 / 12.1 / 12.2, 1024 (4) 49 / 26 / 34 / 28 / 33, 1470 59 / 30 / 31 / 21 / 30,
 // 2048 77 / 41 / 43 / 46 / 77, 2048 (2) - / 83 / 67 / 80 / -, 4096 183 / 239 / 238 / 339 / -, 4096 over 50,176 1974 / 2521 / - / 4531 / -:
 // 4096 is 253 tiles of 192, one for each CU, but 528 of 128, two and a bit; two of 2048 are 506 tiles of 96, two for each.
+// The times are those of split matrices, three products a block; X in fp16 alone, two a block, is cut by the same ones.
 struct TileKind {
     int bm, bn, per_cu;
     double block, more, start;
