@@ -204,3 +204,14 @@ def test_captured_steps_of_channels_last_weights(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(weights[0].detach(), weights[1].detach()), turn
+
+
+@pytest.mark.parametrize("shape", [(1, 5), (5,), (1, 1), (3, 4), (5, 3)])
+def test_a_momentum_of_another_shape_is_not_loaded(shape):
+    weights, first, second = _pair()
+    second.load_state_dict(first.state_dict())
+    before = [second.state[p]["momentum_buffer"].clone() for p in weights]
+    first.state[weights[0]]["momentum_buffer"] = torch.ones(shape)
+    with pytest.raises(ValueError, match="momentum of shape"):
+        second.load_state_dict(first.state_dict())
+    assert all(torch.equal(second.state[p]["momentum_buffer"], b) for p, b in zip(weights, before))

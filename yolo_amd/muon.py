@@ -177,18 +177,21 @@ class Muon(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         # torch casts a loaded state to the types of its weights; momenta stay fp32.  They come from what the last
         # pre-hook leaves, and the first post-hook finds them in place.
-        loaded = {}
+        loaded = []              # (weight, its momentum)
 
         def keep(_, given):
-            loaded.update(given)
-
-        def restore(_):
-            keys = [key for group in loaded["param_groups"] for key in group["params"]]
+            keys = [key for group in given["param_groups"] for key in group["params"]]
             weights = [p for group in self.param_groups for p in group["params"]]
             for key, p in zip(keys, weights):
-                saved = loaded["state"].get(key, {}).get("momentum_buffer")
+                saved = given["state"].get(key, {}).get("momentum_buffer")
                 if saved is not None:
-                    self.state[p]["momentum_buffer"] = torch.empty_like(p, dtype=torch.float32, requires_grad=False).copy_(saved.detach())
+                    if saved.shape != p.shape:
+                        raise ValueError(f"Muon: a momentum of shape {tuple(saved.shape)} for a weight of shape {tuple(p.shape)}")
+                    loaded.append((p, saved))
+
+        def restore(_):
+            for p, saved in loaded:
+                self.state[p]["momentum_buffer"] = torch.empty_like(p, dtype=torch.float32, requires_grad=False).copy_(saved.detach())
 
         hooks = [self.register_load_state_dict_pre_hook(keep), self.register_load_state_dict_post_hook(restore, prepend=True)]
         try:
