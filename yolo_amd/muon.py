@@ -68,8 +68,10 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coeffs: Tuple[float, float, f
 
     Columns lie next to each other and rows at any stride of at least ``cols``; leading axes collapse to one.
     The matrices are held in 22 bits: the result (contiguous, ``out_dtype``) is within about 1e-4 of the exact
-    one (whole matrix, relative; 1e-3 when it is bf16) before its rounding, for matrices of up to a few thousand rows.  Coefficients and steps under which, with singular
-    values s in [0, 1], s^2, |b s^2 + c s^4| or s^2 |a + b s^2 + c s^4| may pass 120 before a step are refused.  A NaN or an infinity makes its whole matrix NaN.  Forward only."""
+    one (whole matrix, relative; 1e-3 when it is bf16) before its rounding, for matrices of up to a few thousand rows.
+    Coefficients and steps under which, with singular values s in [0, 1], s^2, |b s^2 + c s^4| or
+    s^2 |a + b s^2 + c s^4| may pass 120 before a step are refused.  A NaN or an infinity makes its whole matrix
+    NaN.  Forward only."""
     _forward_only(g, "g", "orthogonalize")
     _check_steps(steps, eps)
     _check_numbers(coeffs)
